@@ -149,7 +149,7 @@ def _quantised(x):
     to 448 or below; a row of zeros has scale 1."""
     x = x.float()
     mant, ex = torch.frexp(x.abs().amax(-1, keepdim=True))
-    e = (ex - 9 + (mant > 0.875)).clamp(-126, 127)
+    e = (ex - 9 + (mant > 0.875)).clamp(-124, 127)
     e = torch.where(mant == 0, torch.zeros_like(e), e)
     payload = torch.ldexp(x, -e).to(torch.float8_e4m3fn)
     return payload, (e[..., 0] + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
