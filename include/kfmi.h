@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define KFMI_ABI_VERSION 10
+#define KFMI_ABI_VERSION 11
 
 /* status codes */
 #define KFMI_OK 0
@@ -281,6 +281,169 @@ int kfmi_launch_factored_attention_bf16(const void *q, const void *k, const void
                                         void *kn, int64_t B, int64_t Hq, int64_t Hkv, int64_t S,
                                         int64_t D, float eps, int causal, int bm, int bn,
                                         void *work, int64_t work_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Serving: keys and values kept in a paged cache, attention of single tokens
+ * over it, and the log probabilities of the answer.  No counterpart in the
+ * reference, whose path ends with the prefill.  Forward only.
+ *
+ * A cache is two tensors k_cache and v_cache of num_pages pages, logically
+ * [num_pages, Hkv, page_size, D], with equal strides: any strides (in elements) of
+ * page, head and token that are multiples of 16 bytes, rows of D contiguous.
+ * page_size is a power of two, at least 16.  Slot z is row z % page_size of
+ * page z / page_size.
+ *   KFMI_CACHE_BF16: rows of D bf16 values; k_scale and v_scale are NULL.
+ *   KFMI_CACHE_E4M3: rows of D e4m3 (OCP, no infinities) values and one scale
+ *     2^(byte - 127) per row (E8M0; 255 is NaN), k_scale and v_scale
+ *     [num_pages, Hkv, page_size] bytes: strides of page and head that are
+ *     multiples of 4, rows contiguous, pointers 4-byte aligned.  A row's scale is the
+ *     smallest 2^e, e >= -124, that brings its largest finite magnitude to 448
+ *     or below (1 for a row of zeros), so that dividing by it and multiplying by it are
+ *     exact, and e4m3 * scale is a bf16 value; the division's result is
+ *     rounded to nearest even (to 240 at most where 256 * scale would leave bf16's range);
+ *     infinities and NaN are held as NaN.
+ *
+ * Indices (positions, slots, pages, lengths, ids) are int32, or int64 where
+ * the KFMI_I64_* flag says so.  They are on the device, so a wrong one is not an
+ * error code: no entry point reads or writes out of range for any value,
+ * and what a wrong one reaches is NaN, as each function says.
+ * ------------------------------------------------------------------------- */
+#define KFMI_CACHE_BF16 0
+#define KFMI_CACHE_E4M3 1
+
+#define KFMI_I64_POSITIONS 1
+#define KFMI_I64_SLOTS 2
+#define KFMI_I64_PAGES 4
+#define KFMI_I64_LENGTHS 8
+#define KFMI_I64_IDS 16
+
+typedef struct {
+  const void *q;              /* [B,Hq,S,D] bf16, or NULL: K and V only (gq and qn are then ignored) */
+  const void *k, *v;          /* [B,Hkv,S,D] bf16 */
+  const void *gq, *gk;        /* [D] bf16 */
+  const void *cos, *sin;      /* [table_rows,D] bf16, halves duplicated; both NULL: no RoPE */
+  const void *positions;      /* [B,S]: each token's row of the tables (unused without them) */
+  const void *slots;          /* [B,S]: each token's slot; negative: a padding token, not written */
+  void *qn;                   /* [B,Hq,S,D] bf16, contiguous */
+  void *kn;                   /* [B,Hkv,S,D] bf16, contiguous, or NULL */
+  void *k_cache, *v_cache, *k_scale, *v_scale;
+  int64_t q_stride[3], k_stride[3], v_stride[3]; /* of B, H and S, in elements; multiples of 8 */
+  int64_t position_stride[2], slot_stride[2];    /* of B and S, in elements */
+  int64_t cache_stride[3];                       /* of page, head and token, in elements */
+  int64_t scale_stride[2];                       /* of page and head */
+  int64_t B, Hq, Hkv, S, D, table_rows, num_pages, page_size;
+  double eps;
+  int32_t norm_style, cache_type, index_flags, reserved;
+} kfmi_cache_write_args;
+
+/* Per-head RMSNorm * gamma (+ rotate-half RoPE at each token's own position) of
+ * Q rows into qn and of K rows, and V rows as they are, into the cache, in one
+ * launch.  qn equals kfmi_prepare_bf16's rows at the same positions bit for
+ * bit; K rows are its bf16 rows, for KFMI_CACHE_E4M3 rounded again.  kn, where
+ * given, takes the bf16 K rows too (what a prefill over the same tokens
+ * reads).  qn may be q where q is contiguous; no other operands may
+ * overlap.  A position outside the tables makes the token's qn, kn and cached K rows NaN; a
+ * slot behind the cache makes its qn and kn rows NaN and writes nothing to the cache.  The
+ * slots of one call that are not negative must differ (a slot given twice
+ * holds some mixture of those tokens' rows). */
+int kfmi_norm_rope_to_cache_bf16(const kfmi_cache_write_args *args, void *stream);
+
+typedef struct {
+  const void *q;                             /* [B,Hq,S,D] bf16, prepared (qn of kfmi_norm_rope_to_cache_bf16) */
+  const void *k_cache, *v_cache, *k_scale, *v_scale;
+  const void *pages;                         /* [B,max_pages]: the pages of each sequence, in order */
+  const void *lengths;                       /* [B]: keys of each sequence, its S new tokens among them */
+  void *out;                                 /* [B,Hq,S,D] bf16, contiguous */
+  void *work;                                /* workspace or NULL */
+  int64_t work_bytes;
+  int64_t q_stride[3];                       /* of B, H and S, in elements; multiples of 8 */
+  int64_t cache_stride[3], scale_stride[2];  /* as in kfmi_cache_write_args */
+  int64_t pages_stride, lengths_stride;      /* between sequences, in elements */
+  int64_t B, Hq, Hkv, S, D, num_pages, page_size, max_pages;
+  int64_t window;                            /* keys a query sees, itself among them; 0: all before it */
+  double scale, softcap;                     /* softcap 0: none */
+  int32_t cache_type, index_flags;
+} kfmi_decode_args;
+
+/* Attention of each sequence's last S tokens (1 <= S <= 16) over its paged cache:
+ * query i of sequence b has position t = lengths[b] - S + i and sees the keys
+ * max(0, t - window + 1) .. t (all up to t when window is 0); scores are
+ * (q . k) * scale, then softcap * tanh(score / softcap) when softcap > 0.
+ * A query that sees no key (t < 0) gives zeros.  Entries of
+ * pages behind a sequence's last key or before its window are not read, nor
+ * is a cached row that no query sees; what those hold (NaN, infinities) does not matter.
+ * A length below 0 or above max_pages * page_size, or a page outside the cache among
+ * those that a query sees, makes the sequence's outputs NaN.
+ *
+ * The work is dealt evenly to one round of workgroups whatever the lengths
+ * are, so a long sequence is split over several; their partial results (32-bit) are
+ * joined in order by the workgroup that finishes last, in `work`:
+ * kfmi_attention_decode_workspace bytes, whose first KFMI_DECODE_COUNTER_BYTES the
+ * caller zero-fills once; each launch leaves them at zero.  Calls that share a
+ * workspace must not overlap in time.  With work == NULL or fewer bytes a
+ * sequence's head is never split (slower for few or uneven sequences). */
+int kfmi_attention_decode_bf16(const kfmi_decode_args *args, void *stream);
+
+#define KFMI_DECODE_COUNTER_BYTES 8192
+
+/* Bytes of the workspace of kfmi_attention_decode_bf16 for these arguments (pointers and
+ * strides are ignored) on the current device, into *bytes. */
+int kfmi_attention_decode_workspace(const kfmi_decode_args *args, int64_t *bytes);
+
+typedef struct {
+  const void *k_cache, *v_cache, *k_scale, *v_scale;
+  const void *pages, *lengths;               /* as in kfmi_decode_args */
+  void *k, *v;                               /* [B,Hkv,L,D] bf16, contiguous */
+  int64_t cache_stride[3], scale_stride[2];
+  int64_t pages_stride, lengths_stride;
+  int64_t B, Hkv, L, D, num_pages, page_size, max_pages;
+  int32_t cache_type, index_flags;
+} kfmi_cache_read_args;
+
+/* The first L rows of each sequence's pages as contiguous K and V; an e4m3
+ * row as payload * scale (exact).  Rows behind a sequence's length are
+ * zeros; rows of a page outside the cache are NaN, and so are all rows of a
+ * sequence whose length is below 0 or above max_pages * page_size.  A length above L
+ * gives the first L rows. */
+int kfmi_cache_to_dense_bf16(const kfmi_cache_read_args *args, void *stream);
+
+#define KFMI_LOGITS_F32 0
+#define KFMI_LOGITS_BF16 1
+#define KFMI_LOGITS_F16 2
+
+#define KFMI_LOGPROBS_TOP_MAX 32
+
+typedef struct {
+  const void *logits;           /* [N0,N1,V] */
+  const void *ids;              /* [N0,N1] */
+  float *logprobs, *entropy;    /* [N0,N1] */
+  float *top_logprobs;          /* [N0,N1,top] (top > 0) */
+  int64_t *top_ids;             /* [N0,N1,top] (top > 0) */
+  void *work;
+  int64_t work_bytes;
+  int64_t logits_stride[2], ids_stride[2]; /* of N0 and N1, in elements */
+  int64_t N0, N1, V;
+  int32_t top, logits_type, index_flags, reserved;
+} kfmi_logprobs_args;
+
+/* For each row x of logits (V < 2^31), in one pass over it:
+ *   logprobs = x[id] - log sum exp x        (NaN for an id outside 0 .. V-1)
+ *   entropy  = -sum p log p, p = softmax x  (p = 0 adds nothing)
+ *   top_ids  = the `top` (0 .. 32, at most V) largest logits' indices, largest first,
+ *              equal logits by the lower index; top_logprobs their log probabilities.
+ * A row that holds NaN or +infinity, or nothing but -infinity, has no
+ * distribution: its outputs are NaN and its top_ids -1.
+ * Rows that few workgroups would read alone are split over several, which are joined
+ * through `work` (kfmi_token_logprobs_workspace bytes; the first
+ * KFMI_LOGPROBS_COUNTER_BYTES zero-filled once, left at zero by each launch; calls that share one
+ * must not overlap in time).  With work == NULL or fewer bytes no row is split. */
+int kfmi_token_logprobs(const kfmi_logprobs_args *args, void *stream);
+
+#define KFMI_LOGPROBS_COUNTER_BYTES 8192
+
+/* Bytes of the workspace of kfmi_token_logprobs for these arguments (pointers and strides are
+ * ignored) on the current device, into *bytes. */
+int kfmi_token_logprobs_workspace(const kfmi_logprobs_args *args, int64_t *bytes);
 
 #ifdef __cplusplus
 }

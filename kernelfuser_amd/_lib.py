@@ -8,6 +8,7 @@ binds to (both use the ``libamdhip64.so.7`` soname).
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from collections.abc import Sequence
 from pathlib import Path
@@ -15,7 +16,7 @@ from pathlib import Path
 import torch  # noqa: F401  (loads torch's HIP runtime before the library)
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libkfmi.so"
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 KFMI_OK, KFMI_EINVAL, KFMI_ELAUNCH, KFMI_EDEVICE = 0, 1, 2, 3
 NORM_STYLES = {"hf": 0, "legacy": 1, "fp32": 2}
@@ -30,6 +31,7 @@ _I64 = ctypes.c_int64
 _I = ctypes.c_int
 _F = ctypes.c_float
 _D = ctypes.c_double
+_S = ctypes.c_char_p
 
 # name -> argtypes (restype is int for all compute entry points)
 SIGNATURES = {
@@ -46,7 +48,27 @@ SIGNATURES = {
                                      _I64, _P],
     "kfmi_launch_factored_attention_bf16": [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _F, _I,
                                             _I, _I, _P, _I64, _P],
+    # a packed argument structure (bytes of its struct.Struct below), then the stream
+    "kfmi_norm_rope_to_cache_bf16": [_S, _P],
+    "kfmi_attention_decode_bf16": [_S, _P],
+    "kfmi_attention_decode_workspace": [_S, ctypes.POINTER(_I64)],
+    "kfmi_cache_to_dense_bf16": [_S, _P],
+    "kfmi_token_logprobs": [_S, _P],
+    "kfmi_token_logprobs_workspace": [_S, ctypes.POINTER(_I64)],
 }
+
+# The argument structures of the serving entry points (kfmi_*_args), in the
+# order of their fields: P pointer, q int64, d double, i int32.  Packing bytes costs
+# about a microsecond; filling a ctypes.Structure field by field five times that.
+CACHE_WRITE_ARGS = struct.Struct("15P" "18q" "8q" "d" "4i")
+DECODE_ARGS = struct.Struct("9P" "q" "8q" "2q" "8q" "q" "2d" "2i")
+CACHE_READ_ARGS = struct.Struct("8P" "5q" "2q" "7q" "2i")
+LOGPROBS_ARGS = struct.Struct("7P" "q" "4q" "3q" "4i")
+
+CACHE_BF16, CACHE_E4M3 = 0, 1
+I64_POSITIONS, I64_SLOTS, I64_PAGES, I64_LENGTHS, I64_IDS = 1, 2, 4, 8, 16
+LOGITS_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+LOGPROBS_TOP_MAX = 32
 
 _lock = threading.Lock()
 _lib = None

@@ -1,0 +1,302 @@
+// The paged key-value cache: rows prepared and written into it, and its pages
+// read back as dense tensors (the layout is described in kfmi.h).
+//
+// Both are memory-bound: a row of D values is D/8 lanes of 8 values each (one
+// 16-lane DPP row at D = 128), 16 bytes of bf16 or 8 bytes of e4m3 per lane.
+#include <cstdio>
+#include <string>
+
+#include "cache_common.h"
+#include "kfmi_launch.h"
+#include "rows_common.h"
+
+namespace kfmi {
+namespace {
+
+struct WriteParams {
+  const uint16_t *q, *k, *v, *gq, *gk, *cos, *sin;
+  const void *positions, *slots;
+  uint16_t *qn, *kn;
+  char *k_cache, *v_cache;
+  uint8_t *k_scale, *v_scale;
+  int64_t qs[3], ks[3], vs[3];  // strides of B, H, S in elements
+  int64_t ps[2], ss[2];
+  int64_t cs[3], es[2];
+  uint32_t S, T, hq, hk;  // T = B * S tokens; heads of q (0: none) and of k
+  uint32_t rows;          // T * (hq + 2 * hk)
+  int64_t table_rows, slot_end;
+  int page_shift, page_mask;
+  bool pos64, slot64;
+  float eps;
+};
+
+// A row of 8 values per lane in e4m3 with its scale 2^e: e is the smallest
+// exponent (at least -124: e4m3's smallest step, 2^-9, times 2^-124 is bf16's) with max|row| <= 448 * 2^e over the finite values, so that the
+// division by the scale is exact and the conversion (round to nearest even)
+// cannot overflow.  448 = 0.875 * 2^9: with max = m * 2^x, 0.5 <= m < 1, e is
+// x - 9, one more where m > 0.875.  Only at e = 120 could a rounding up (to
+// 256 * 2^120 = 2^128) leave bf16's range: 240 is the most there.  Returns the
+// payload; byte = e + 127.
+template <int LPR>
+__device__ __forceinline__ u32x2_t quantise_row(const float (&y)[8], uint32_t &byte) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t a = __float_as_uint(y[j]) & 0x7fffffffu;
+    top = max(top, a < 0x7f800000u ? a : 0u);
+  }
+  top = row_max_u32<LPR>(top);
+  const int ex = (int)(top >> 23) - 126 - 9 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  const int e = top == 0 ? 0 : max(ex, -124);
+  byte = (uint32_t)(e + 127);
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+  const float most = e == 120 ? 240.0f : 448.0f;
+  float z[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    z[j] = __builtin_amdgcn_fmed3f(y[j] * inv, -most, most);
+    if ((__float_as_uint(y[j]) & 0x7f800000u) == 0x7f800000u) z[j] = __uint_as_float(0x7fc00000u);
+  }
+  u32x2_t w;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int x = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * i], z[4 * i + 1], 0, false);
+    x = __builtin_amdgcn_cvt_pk_fp8_f32(z[4 * i + 2], z[4 * i + 3], x, true);
+    w[i] = (uint32_t)x;
+  }
+  return w;
+}
+
+// One row per LPR lanes; rows in the order (head, token), heads of q, then k,
+// then v, so that neighbouring rows are neighbouring tokens of one head (or, for a few
+// tokens, neighbouring heads).
+template <int D, int ST, bool ROPE, bool FP8>
+__global__ __launch_bounds__(256) void cache_write_kernel(WriteParams p) {
+  constexpr int LPR = D / 8;
+  constexpr int HALF = LPR / 2;
+  const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const uint32_t lc = threadIdx.x % LPR;
+  const bool live = row < p.rows;
+  const uint32_t r = live ? row : p.rows - 1;  // loads stay in bounds; nothing is stored for this lane
+  const uint32_t head = r / p.T, t = r - head * p.T;
+  const uint32_t b = t / p.S, s = t - b * p.S;
+  const bool is_q = head < p.hq, is_v = head >= p.hq + p.hk;
+  const uint32_t h = is_q ? head : is_v ? head - p.hq - p.hk : head - p.hq;
+  const uint16_t *src = is_q ? p.q : is_v ? p.v : p.k;
+  const int64_t s0 = is_q ? p.qs[0] : is_v ? p.vs[0] : p.ks[0];
+  const int64_t s1 = is_q ? p.qs[1] : is_v ? p.vs[1] : p.ks[1];
+  const int64_t s2 = is_q ? p.qs[2] : is_v ? p.vs[2] : p.ks[2];
+  const u32x4_t xw = ld16_nt(src + b * s0 + h * s1 + s * s2 + lc * 8);
+  const int64_t slot = load_index(p.slots, p.slot64, b * p.ss[0] + s * p.ss[1]);
+  const u32x4_t gw = ld16((is_q ? p.gq : p.gk) + lc * 8);
+  bool bad_pos = false;
+  u32x4_t cw, sw;
+  if constexpr (ROPE) {
+    int64_t pos = load_index(p.positions, p.pos64, b * p.ps[0] + s * p.ps[1]);
+    bad_pos = pos < 0 || pos >= p.table_rows;
+    pos = bad_pos ? 0 : pos;
+    cw = ld16(p.cos + pos * D + lc * 8);
+    sw = ld16(p.sin + pos * D + lc * 8);
+  }
+  const bool bad_slot = slot >= p.slot_end;
+  float x[8], y[8];
+  unpack8(xw, x);
+  float g[8];
+  unpack8(gw, g);
+  const float inv = row_inv_rms<LPR, D>(x, p.eps);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) y[j] = norm_elem<ST>(x[j], inv, g[j]);
+  if constexpr (ROPE) {
+    const uint32_t flip = lc < HALF ? 0x80008000u : 0u;  // first half: n*c - np*s
+    sw ^= u32x4_t{flip, flip, flip, flip};
+    float c[8], sn[8];
+    unpack8(cw, c);
+    unpack8(sw, sn);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = rope_elem<ST>(y[j], partner_f32<LPR>(y[j]), c[j], sn[j], false);
+  }
+  u32x4_t yw = pack8(y);
+  const uint32_t nan2 = 0x7fc07fc0u;
+  if (bad_pos) yw = u32x4_t{nan2, nan2, nan2, nan2};
+  const u32x4_t held = is_v ? xw : yw;  // what the cache holds
+  u32x2_t payload;
+  uint32_t byte = 0;
+  if constexpr (FP8) {
+    float f[8];
+    unpack8(held, f);
+    payload = quantise_row<LPR>(f, byte);
+  }
+  if (!live) return;
+  if (!is_v && (is_q || p.kn)) {
+    if (bad_slot) yw = u32x4_t{nan2, nan2, nan2, nan2};
+    uint16_t *dst = is_q ? p.qn : p.kn;
+    const uint32_t nh = is_q ? p.hq : p.hk;
+    st16_nt(dst + (((int64_t)b * nh + h) * p.S + s) * D + lc * 8, yw);
+  }
+  if (is_q || slot < 0 || bad_slot) return;
+  const int64_t page = slot >> p.page_shift, at = slot & p.page_mask;
+  const int64_t off = page * p.cs[0] + h * p.cs[1] + at * p.cs[2] + lc * 8;
+  char *cache = is_v ? p.v_cache : p.k_cache;
+  if constexpr (FP8) {
+    *reinterpret_cast<u32x2_t *>(cache + off) = payload;
+    if (lc == 0) (is_v ? p.v_scale : p.k_scale)[page * p.es[0] + h * p.es[1] + at] = (uint8_t)byte;
+  } else {
+    st16(reinterpret_cast<uint16_t *>(cache) + off, held);
+  }
+}
+
+template <int D, int ST, bool ROPE, bool FP8>
+hipError_t launch_write_t(const WriteParams &p, hipStream_t stream) {
+  const int64_t grid = ((int64_t)p.rows + 256 / (D / 8) - 1) / (256 / (D / 8));
+  hipLaunchKernelGGL((cache_write_kernel<D, ST, ROPE, FP8>), dim3((unsigned)grid), dim3(256), 0, stream, p);
+  static const std::string name = [] {
+    char b[96];
+    snprintf(b, sizeof(b), "cache_write_kernel<%d, %d, %s, %s>", D, ST, tf(ROPE), tf(FP8));
+    return std::string(b);
+  }();
+  launch_log_add(reinterpret_cast<const void *>(&cache_write_kernel<D, ST, ROPE, FP8>), name.c_str(), grid, 256);
+  return hipGetLastError();
+}
+
+template <int D, int ST>
+hipError_t dispatch_write(const WriteParams &p, bool rope, bool fp8, hipStream_t s) {
+  if (rope) return fp8 ? launch_write_t<D, ST, true, true>(p, s) : launch_write_t<D, ST, true, false>(p, s);
+  return fp8 ? launch_write_t<D, ST, false, true>(p, s) : launch_write_t<D, ST, false, false>(p, s);
+}
+
+struct ReadParams {
+  const char *k_cache, *v_cache;
+  const uint8_t *k_scale, *v_scale;
+  const void *pages, *lengths;
+  uint16_t *k, *v;
+  int64_t cs[3], es[2];
+  int64_t pages_stride, lengths_stride, num_pages, capacity;
+  uint32_t L, hk, rows_per_seq;  // hk * L
+  int page_shift, page_mask;
+  bool pages64, len64;
+};
+
+// One row of K and of V per LPR lanes: row (h, j) of sequence blockIdx.y.
+template <int D, bool FP8>
+__global__ __launch_bounds__(256) void cache_read_kernel(ReadParams p) {
+  constexpr int LPR = D / 8;
+  const int64_t b = blockIdx.y;
+  const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const uint32_t lc = threadIdx.x % LPR;
+  if (row >= p.rows_per_seq) return;
+  const uint32_t h = row / p.L, j = row - h * p.L;
+  const int64_t len = load_index(p.lengths, p.len64, b * p.lengths_stride);
+  const uint32_t nan2 = 0x7fc07fc0u;
+  u32x4_t out[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
+  bool bad = len < 0 || len > p.capacity;
+  if (!bad && j < len) {
+    const int64_t page = load_index(p.pages, p.pages64, b * p.pages_stride + (j >> p.page_shift));
+    bad = page < 0 || page >= p.num_pages;
+    if (!bad) {
+      const int64_t at = j & p.page_mask;
+      const int64_t off = page * p.cs[0] + h * p.cs[1] + at * p.cs[2] + lc * 8;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const char *c = i ? p.v_cache : p.k_cache;
+        if constexpr (FP8) {
+          const u32x2_t w = *reinterpret_cast<const u32x2_t *>(c + off);
+          const float sc = scale_value((i ? p.v_scale : p.k_scale)[page * p.es[0] + h * p.es[1] + at]);
+          float f[8];
+          unpack_e4m3(w, f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] *= sc;
+          out[i] = pack8(f);
+        } else {
+          out[i] = ld16(reinterpret_cast<const uint16_t *>(c) + off);
+        }
+      }
+    }
+  }
+  if (bad) out[0] = out[1] = u32x4_t{nan2, nan2, nan2, nan2};
+  const int64_t o = (b * p.rows_per_seq + row) * D + lc * 8;
+  st16_nt(p.k + o, out[0]);
+  st16_nt(p.v + o, out[1]);
+}
+
+template <int D, bool FP8>
+hipError_t launch_read_t(const ReadParams &p, int64_t B, hipStream_t stream) {
+  const dim3 grid((p.rows_per_seq + 256 / (D / 8) - 1) / (256 / (D / 8)), (unsigned)B);
+  hipLaunchKernelGGL((cache_read_kernel<D, FP8>), grid, dim3(256), 0, stream, p);
+  static const std::string name = [] {
+    char b[96];
+    snprintf(b, sizeof(b), "cache_read_kernel<%d, %s>", D, tf(FP8));
+    return std::string(b);
+  }();
+  launch_log_add(reinterpret_cast<const void *>(&cache_read_kernel<D, FP8>), name.c_str(), (int64_t)grid.x * grid.y, 256);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_cache_write(const kfmi_cache_write_args &a, int style, hipStream_t stream) {
+  WriteParams p{};
+  p.q = (const uint16_t *)a.q; p.k = (const uint16_t *)a.k; p.v = (const uint16_t *)a.v;
+  p.gq = (const uint16_t *)a.gq; p.gk = (const uint16_t *)a.gk;
+  p.cos = (const uint16_t *)a.cos; p.sin = (const uint16_t *)a.sin;
+  p.positions = a.positions; p.slots = a.slots;
+  p.qn = (uint16_t *)a.qn; p.kn = (uint16_t *)a.kn;
+  p.k_cache = (char *)a.k_cache; p.v_cache = (char *)a.v_cache;
+  p.k_scale = (uint8_t *)a.k_scale; p.v_scale = (uint8_t *)a.v_scale;
+  for (int i = 0; i < 3; ++i) {
+    p.qs[i] = a.q_stride[i]; p.ks[i] = a.k_stride[i]; p.vs[i] = a.v_stride[i]; p.cs[i] = a.cache_stride[i];
+  }
+  for (int i = 0; i < 2; ++i) {
+    p.ps[i] = a.position_stride[i]; p.ss[i] = a.slot_stride[i]; p.es[i] = a.scale_stride[i];
+  }
+  p.S = (uint32_t)a.S;
+  p.T = (uint32_t)(a.B * a.S);
+  p.hq = a.q ? (uint32_t)a.Hq : 0u;
+  p.hk = (uint32_t)a.Hkv;
+  p.rows = p.T * (p.hq + 2 * p.hk);
+  p.table_rows = a.table_rows;
+  p.slot_end = a.num_pages * a.page_size;
+  p.page_shift = log2_of(a.page_size);
+  p.page_mask = (int)(a.page_size - 1);
+  p.pos64 = a.index_flags & KFMI_I64_POSITIONS;
+  p.slot64 = a.index_flags & KFMI_I64_SLOTS;
+  p.eps = (float)a.eps;
+  const bool rope = a.cos != nullptr, fp8 = a.cache_type == KFMI_CACHE_E4M3;
+#define KFMI_STYLES(D)                                                 \
+  switch (style) {                                                     \
+    case ST_HF: return dispatch_write<D, ST_HF>(p, rope, fp8, stream); \
+    case ST_LEGACY: return dispatch_write<D, ST_LEGACY>(p, rope, fp8, stream); \
+    case ST_FP32: return dispatch_write<D, ST_FP32>(p, rope, fp8, stream); \
+  }
+  if (a.D == 128) {
+    KFMI_STYLES(128)
+  } else {
+    KFMI_STYLES(256)
+  }
+#undef KFMI_STYLES
+  return hipErrorInvalidValue;
+}
+
+hipError_t launch_cache_read(const kfmi_cache_read_args &a, hipStream_t stream) {
+  ReadParams p{};
+  p.k_cache = (const char *)a.k_cache; p.v_cache = (const char *)a.v_cache;
+  p.k_scale = (const uint8_t *)a.k_scale; p.v_scale = (const uint8_t *)a.v_scale;
+  p.pages = a.pages; p.lengths = a.lengths;
+  p.k = (uint16_t *)a.k; p.v = (uint16_t *)a.v;
+  for (int i = 0; i < 3; ++i) p.cs[i] = a.cache_stride[i];
+  for (int i = 0; i < 2; ++i) p.es[i] = a.scale_stride[i];
+  p.pages_stride = a.pages_stride; p.lengths_stride = a.lengths_stride;
+  p.num_pages = a.num_pages;
+  p.capacity = a.max_pages * a.page_size;
+  p.L = (uint32_t)a.L;
+  p.hk = (uint32_t)a.Hkv;
+  p.rows_per_seq = p.hk * p.L;
+  p.page_shift = log2_of(a.page_size);
+  p.page_mask = (int)(a.page_size - 1);
+  p.pages64 = a.index_flags & KFMI_I64_PAGES;
+  p.len64 = a.index_flags & KFMI_I64_LENGTHS;
+  const bool fp8 = a.cache_type == KFMI_CACHE_E4M3;
+  if (a.D == 128) return fp8 ? launch_read_t<128, true>(p, a.B, stream) : launch_read_t<128, false>(p, a.B, stream);
+  return fp8 ? launch_read_t<256, true>(p, a.B, stream) : launch_read_t<256, false>(p, a.B, stream);
+}
+
+}  // namespace kfmi

@@ -464,4 +464,175 @@ int kfmi_launch_factored_attention_bf16(const void *q, const void *k, const void
                         kfmi::PRO_FACTORED_CALC, kfmi::ST_FP32, bm, bn, (hipStream_t)stream, work, work_bytes);
 }
 
+// ---------------------------------------------------------------------------
+// Serving entry points
+// ---------------------------------------------------------------------------
+
+static int check_aligned(const void *p, uintptr_t to, const char *name) {
+  if (p == nullptr) return fail(KFMI_EINVAL, "%s must not be NULL", name);
+  if (reinterpret_cast<uintptr_t>(p) & (to - 1)) return fail(KFMI_EINVAL, "%s must be %d-byte aligned", name, (int)to);
+  return KFMI_OK;
+}
+
+// check_shape for sizes that come in a structure: each below 2^31 and the elements
+// counted factor by factor, so that no product leaves 64 bits.
+static int check_sizes(int64_t B, int64_t Hq, int64_t Hkv, int64_t S, int64_t D) {
+  const int64_t lim = (int64_t)1 << 31, dims[] = {B, Hq > Hkv ? Hq : Hkv, S, D};
+  int64_t n = 1;
+  for (int64_t d : dims) {
+    if (d >= lim || (d > 0 && n * d >= lim)) return fail(KFMI_EINVAL, "tensors must have fewer than 2^31 elements");
+    n *= d > 0 ? d : 1;
+  }
+  return check_shape(B, Hq, Hkv, S, D);
+}
+
+static int check_index(const void *p, int flags, int flag, const char *name) {
+  return check_aligned(p, flags & flag ? 8 : 4, name);
+}
+
+static int check_strides(const int64_t *strides, int n, int64_t of, const char *name) {
+  for (int i = 0; i < n; ++i)
+    if (strides[i] % of != 0) return fail(KFMI_EINVAL, "%s strides must be multiples of %lld elements", name, (long long)of);
+  return KFMI_OK;
+}
+
+// The pages, rows and scales of a cache (kfmi.h).
+static int check_cache(const void *k, const void *v, const void *ks, const void *vs, const int64_t *cs,
+                       const int64_t *es, int64_t num_pages, int64_t page_size, int cache_type) {
+  if (cache_type != KFMI_CACHE_BF16 && cache_type != KFMI_CACHE_E4M3)
+    return fail(KFMI_EINVAL, "cache_type must be KFMI_CACHE_BF16 or KFMI_CACHE_E4M3 (got %d)", cache_type);
+  if (num_pages < 1) return fail(KFMI_EINVAL, "num_pages must be >= 1 (got %lld)", (long long)num_pages);
+  if (page_size < 16 || page_size > (1 << 20) || (page_size & (page_size - 1)))
+    return fail(KFMI_EINVAL, "page_size must be a power of two from 16 to 2^20 (got %lld)", (long long)page_size);
+  if (num_pages > ((int64_t)1 << 62) / page_size) return fail(KFMI_EINVAL, "too many pages");
+  KFMI_TRY(check_ptrs({{k, "k_cache"}, {v, "v_cache"}}));
+  KFMI_TRY(check_strides(cs, 3, cache_type == KFMI_CACHE_E4M3 ? 16 : 8, "cache"));
+  if (cache_type == KFMI_CACHE_E4M3) {
+    KFMI_TRY(check_aligned(ks, 4, "k_scale"));
+    KFMI_TRY(check_aligned(vs, 4, "v_scale"));
+    KFMI_TRY(check_strides(es, 2, 4, "scale"));
+  } else if (ks || vs) {
+    return fail(KFMI_EINVAL, "a bf16 cache has no scales");
+  }
+  return KFMI_OK;
+}
+
+int kfmi_norm_rope_to_cache_bf16(const kfmi_cache_write_args *a, void *stream) {
+  if (a == nullptr) return fail(KFMI_EINVAL, "args must not be NULL");
+  KFMI_TRY(check_sizes(a->B, a->q ? a->Hq : a->Hkv, a->Hkv, a->S, a->D));
+  KFMI_TRY(check_style(a->norm_style));
+  if (a->index_flags & ~(KFMI_I64_POSITIONS | KFMI_I64_SLOTS)) return fail(KFMI_EINVAL, "unknown index_flags 0x%x", a->index_flags);
+  KFMI_TRY(check_ptrs({{a->k, "k"}, {a->v, "v"}, {a->gk, "gk"}}));
+  KFMI_TRY(check_strides(a->k_stride, 3, 8, "k"));
+  KFMI_TRY(check_strides(a->v_stride, 3, 8, "v"));
+  if (a->q) {
+    KFMI_TRY(check_ptrs({{a->q, "q"}, {a->gq, "gq"}, {a->qn, "qn"}}));
+    KFMI_TRY(check_strides(a->q_stride, 3, 8, "q"));
+  }
+  if (a->kn) KFMI_TRY(check_ptrs({{a->kn, "kn"}}));
+  if ((a->cos == nullptr) != (a->sin == nullptr)) return fail(KFMI_EINVAL, "provide both rotary tables or neither");
+  if (a->cos) {
+    KFMI_TRY(check_ptrs({{a->cos, "cos"}, {a->sin, "sin"}}));
+    KFMI_TRY(check_index(a->positions, a->index_flags, KFMI_I64_POSITIONS, "positions"));
+    if (a->table_rows < 1) return fail(KFMI_EINVAL, "table_rows must be >= 1 (got %lld)", (long long)a->table_rows);
+  }
+  KFMI_TRY(check_index(a->slots, a->index_flags, KFMI_I64_SLOTS, "slots"));
+  KFMI_TRY(check_cache(a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->cache_stride, a->scale_stride, a->num_pages,
+                       a->page_size, a->cache_type));
+  if (!(a->eps >= 0.0)) return fail(KFMI_EINVAL, "eps must be >= 0");
+  KFMI_TRY(check_device());
+  return launch_status(kfmi::launch_cache_write(*a, style_of(a->norm_style), (hipStream_t)stream), "cache write launch");
+}
+
+static int check_decode_shape(const kfmi_decode_args *a) {
+  if (a == nullptr) return fail(KFMI_EINVAL, "args must not be NULL");
+  KFMI_TRY(check_sizes(a->B, a->Hq, a->Hkv, a->S, a->D));
+  if (a->S > 16) return fail(KFMI_EINVAL, "S must be at most 16 (got %lld)", (long long)a->S);
+  if (a->B > 65535) return fail(KFMI_EINVAL, "B must be at most 65535 (got %lld)", (long long)a->B);
+  if (a->max_pages < 1) return fail(KFMI_EINVAL, "max_pages must be >= 1 (got %lld)", (long long)a->max_pages);
+  if (a->page_size < 1 || a->max_pages > ((int64_t)1 << 31) / a->page_size)
+    return fail(KFMI_EINVAL, "a sequence's pages must hold at most 2^31 keys");
+  return KFMI_OK;
+}
+
+int kfmi_attention_decode_bf16(const kfmi_decode_args *a, void *stream) {
+  KFMI_TRY(check_decode_shape(a));
+  if (a->index_flags & ~(KFMI_I64_PAGES | KFMI_I64_LENGTHS)) return fail(KFMI_EINVAL, "unknown index_flags 0x%x", a->index_flags);
+  KFMI_TRY(check_ptrs({{a->q, "q"}, {a->out, "out"}}));
+  KFMI_TRY(check_strides(a->q_stride, 3, 8, "q"));
+  KFMI_TRY(check_index(a->pages, a->index_flags, KFMI_I64_PAGES, "pages"));
+  KFMI_TRY(check_index(a->lengths, a->index_flags, KFMI_I64_LENGTHS, "lengths"));
+  KFMI_TRY(check_cache(a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->cache_stride, a->scale_stride, a->num_pages,
+                       a->page_size, a->cache_type));
+  if (!(a->scale > 0.0)) return fail(KFMI_EINVAL, "scale must be > 0");
+  if (!(a->softcap >= 0.0)) return fail(KFMI_EINVAL, "softcap must be >= 0");
+  if (a->window < 0) return fail(KFMI_EINVAL, "window must be >= 0 (got %lld)", (long long)a->window);
+  KFMI_TRY(check_work(a->work, a->work_bytes));
+  KFMI_TRY(check_device());
+  return launch_status(kfmi::launch_decode(*a, (hipStream_t)stream), "decode launch");
+}
+
+int kfmi_attention_decode_workspace(const kfmi_decode_args *a, int64_t *bytes) {
+  if (bytes == nullptr) return fail(KFMI_EINVAL, "bytes must not be NULL");
+  KFMI_TRY(check_decode_shape(a));
+  g_error.clear();
+  *bytes = kfmi::decode_workspace_bytes(*a);
+  return KFMI_OK;
+}
+
+int kfmi_cache_to_dense_bf16(const kfmi_cache_read_args *a, void *stream) {
+  if (a == nullptr) return fail(KFMI_EINVAL, "args must not be NULL");
+  KFMI_TRY(check_sizes(a->B, a->Hkv, a->Hkv, a->L, a->D));
+  if (a->B > 65535) return fail(KFMI_EINVAL, "B must be at most 65535 (got %lld)", (long long)a->B);
+  if (a->max_pages < 1) return fail(KFMI_EINVAL, "max_pages must be >= 1 (got %lld)", (long long)a->max_pages);
+  if (a->index_flags & ~(KFMI_I64_PAGES | KFMI_I64_LENGTHS)) return fail(KFMI_EINVAL, "unknown index_flags 0x%x", a->index_flags);
+  KFMI_TRY(check_index(a->pages, a->index_flags, KFMI_I64_PAGES, "pages"));
+  KFMI_TRY(check_index(a->lengths, a->index_flags, KFMI_I64_LENGTHS, "lengths"));
+  KFMI_TRY(check_cache(a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->cache_stride, a->scale_stride, a->num_pages,
+                       a->page_size, a->cache_type));
+  if (a->max_pages > ((int64_t)1 << 31) / a->page_size)
+    return fail(KFMI_EINVAL, "a sequence's pages must hold at most 2^31 keys");
+  KFMI_TRY(check_ptrs({{a->k, "k"}, {a->v, "v"}}));
+  KFMI_TRY(check_device());
+  return launch_status(kfmi::launch_cache_read(*a, (hipStream_t)stream), "cache read launch");
+}
+
+static int check_logprobs_shape(const kfmi_logprobs_args *a) {
+  if (a == nullptr) return fail(KFMI_EINVAL, "args must not be NULL");
+  if (a->N0 < 1 || a->N1 < 1 || a->V < 1)
+    return fail(KFMI_EINVAL, "N0, N1 and V must be >= 1 (got %lld, %lld, %lld)", (long long)a->N0, (long long)a->N1, (long long)a->V);
+  const int64_t lim = (int64_t)1 << 31;
+  if (a->V >= lim || a->N0 >= lim || a->N1 >= lim || a->N0 * a->N1 >= lim / 64)
+    return fail(KFMI_EINVAL, "V must be below 2^31 and N0 * N1 below 2^25");
+  if (a->logits_type < KFMI_LOGITS_F32 || a->logits_type > KFMI_LOGITS_F16)
+    return fail(KFMI_EINVAL, "logits_type must be KFMI_LOGITS_F32, _BF16 or _F16 (got %d)", a->logits_type);
+  if (a->top < 0 || a->top > KFMI_LOGPROBS_TOP_MAX || a->top > a->V)
+    return fail(KFMI_EINVAL, "top must be from 0 to %d and at most V (got %d)", KFMI_LOGPROBS_TOP_MAX, a->top);
+  return KFMI_OK;
+}
+
+int kfmi_token_logprobs(const kfmi_logprobs_args *a, void *stream) {
+  KFMI_TRY(check_logprobs_shape(a));
+  if (a->index_flags & ~KFMI_I64_IDS) return fail(KFMI_EINVAL, "unknown index_flags 0x%x", a->index_flags);
+  KFMI_TRY(check_aligned(a->logits, a->logits_type == KFMI_LOGITS_F32 ? 4 : 2, "logits"));
+  KFMI_TRY(check_index(a->ids, a->index_flags, KFMI_I64_IDS, "ids"));
+  KFMI_TRY(check_aligned(a->logprobs, 4, "logprobs"));
+  KFMI_TRY(check_aligned(a->entropy, 4, "entropy"));
+  if (a->top > 0) {
+    KFMI_TRY(check_aligned(a->top_logprobs, 4, "top_logprobs"));
+    KFMI_TRY(check_aligned(a->top_ids, 8, "top_ids"));
+  }
+  KFMI_TRY(check_work(a->work, a->work_bytes));
+  KFMI_TRY(check_device());
+  return launch_status(kfmi::launch_logprobs(*a, (hipStream_t)stream), "logprobs launch");
+}
+
+int kfmi_token_logprobs_workspace(const kfmi_logprobs_args *a, int64_t *bytes) {
+  if (bytes == nullptr) return fail(KFMI_EINVAL, "bytes must not be NULL");
+  KFMI_TRY(check_logprobs_shape(a));
+  g_error.clear();
+  *bytes = kfmi::logprobs_workspace_bytes(*a);
+  return KFMI_OK;
+}
+
 }  // extern "C"

@@ -64,6 +64,14 @@ void launch_log_plan(const char *fmt, ...);
 inline const char *tf(bool b) { return b ? "true" : "false"; }
 
 hipError_t launch_rows(const RowsArgs &a, hipStream_t stream);
+// The serving kernels (arguments as in kfmi.h, validated by the caller;
+// `style` is a Style).
+hipError_t launch_cache_write(const kfmi_cache_write_args &a, int style, hipStream_t stream);
+hipError_t launch_cache_read(const kfmi_cache_read_args &a, hipStream_t stream);
+hipError_t launch_decode(const kfmi_decode_args &a, hipStream_t stream);
+int64_t decode_workspace_bytes(const kfmi_decode_args &a);
+hipError_t launch_logprobs(const kfmi_logprobs_args &a, hipStream_t stream);
+int64_t logprobs_workspace_bytes(const kfmi_logprobs_args &a);
 // vt[b,h,d,s] = v[b,h,s,d] for the B*H heads of S rows of D.
 hipError_t launch_transpose_v(const uint16_t *v, uint16_t *vt, int64_t BH, int64_t S, int64_t D, hipStream_t stream);
 hipError_t launch_attention(const AttnArgs &a, hipStream_t stream);

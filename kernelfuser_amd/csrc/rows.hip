@@ -18,6 +18,7 @@
 
 #include "kfmi_device.h"
 #include "kfmi_launch.h"
+#include "rows_common.h"
 
 namespace kfmi {
 namespace {
@@ -90,36 +91,6 @@ __device__ __forceinline__ void transpose_tile(const uint16_t *__restrict__ v, u
   }
 }
 
-// Normalised element x*inv*gamma with the rounding points of a style.
-template <int ST>
-__device__ __forceinline__ float norm_elem(float x, float inv, float g) {
-  if (ST == ST_HF) return round_bf16(round_bf16(x * inv) * g);  // rope:560-561
-  if (ST == ST_LEGACY) return round_bf16(__fmul_rn(__fmul_rn(x, inv), g));  // rope:563
-  return __fmul_rn(__fmul_rn(x, inv), g);  // FP32: rope:125, rope:298
-}
-
-// rotate-half output of one element: first half n*c - np*s, second half n*c + np*s.
-template <int ST>
-__device__ __forceinline__ float rope_elem(float n, float np, float c, float s, bool first) {
-  if (ST == ST_FP32) {  // rope:129 / rope:164-167 (fp32=True): two products, one add
-    // No contraction into an FMA: both products are rounded, then the sum
-    // (HIP's __fmul_rn/__fadd_rn are plain * and + that the headers let the
-    // compiler contract, so the operators are written here).
-#pragma clang fp contract(off)
-    const float p0 = n * c, p1 = np * s;
-    return first ? p0 - p1 : p0 + p1;
-  }
-  float p0 = round_bf16(n * c), p1 = round_bf16(np * s);  // rope:578-579
-  return first ? p0 - p1 : p0 + p1;  // rounded to BF16 at the store (rope:580-581)
-}
-
-template <int LPR>
-__device__ __forceinline__ float row_sum(float x) {
-  x = sum16(x);
-  if constexpr (LPR == 32) x += __shfl_xor(x, 16);
-  return x;
-}
-
 #ifndef KFMI_ROWS_NT
 #define KFMI_ROWS_NT 1
 #endif
@@ -141,13 +112,6 @@ constexpr int64_t ROWS_MID_MIN = (int64_t)1 << 15, ROWS_MID_END = (int64_t)1 << 
 __device__ __forceinline__ u32x4_t ld_row(const uint16_t *p) { return KFMI_ROWS_NT ? ld16_nt(p) : ld16(p); }
 __device__ __forceinline__ void st_row(uint16_t *p, const u32x4_t &v) {
   if (KFMI_ROWS_NT) st16_nt(p, v); else st16(p, v);
-}
-
-// Normalised value held by the rotate-half partner lane (lane ^ LPR/2).
-template <int LPR>
-__device__ __forceinline__ float partner_f32(float x) {
-  if constexpr (LPR == 16) return dpp_f32<DPP_ROW_ROR8>(x);
-  else return __shfl_xor(x, LPR / 2);
 }
 
 // A workgroup of 256 threads covers 256/LPR consecutive positions of HPW
