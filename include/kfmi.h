@@ -372,6 +372,8 @@ typedef struct {
  * A query that sees no key (t < 0) gives zeros.  Entries of
  * pages behind a sequence's last key or before its window are not read, nor
  * is a cached row that no query sees; what those hold (NaN, infinities) does not matter.
+ * A V row with a value that is not finite makes the outputs of the queries that see
+ * it what the formula gives, or, where only some of the S queries see it, NaN throughout.
  * A length below 0 or above max_pages * page_size, or a page outside the cache among
  * those that a query sees, makes the sequence's outputs NaN.
  *

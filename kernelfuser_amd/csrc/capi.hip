@@ -492,7 +492,8 @@ static int check_index(const void *p, int flags, int flag, const char *name) {
 
 static int check_strides(const int64_t *strides, int n, int64_t of, const char *name) {
   for (int i = 0; i < n; ++i)
-    if (strides[i] % of != 0) return fail(KFMI_EINVAL, "%s strides must be multiples of %lld elements", name, (long long)of);
+    if (strides[i] < 0 || strides[i] % of != 0)
+      return fail(KFMI_EINVAL, "%s strides must be multiples of %lld elements", name, (long long)of);
   return KFMI_OK;
 }
 
@@ -507,6 +508,7 @@ static int check_cache(const void *k, const void *v, const void *ks, const void 
   if (num_pages > ((int64_t)1 << 62) / page_size) return fail(KFMI_EINVAL, "too many pages");
   KFMI_TRY(check_ptrs({{k, "k_cache"}, {v, "v_cache"}}));
   KFMI_TRY(check_strides(cs, 3, cache_type == KFMI_CACHE_E4M3 ? 16 : 8, "cache"));
+  if (cs[2] >= (1 << 24)) return fail(KFMI_EINVAL, "the cache's stride between tokens must be below 2^24 elements");
   if (cache_type == KFMI_CACHE_E4M3) {
     KFMI_TRY(check_aligned(ks, 4, "k_scale"));
     KFMI_TRY(check_aligned(vs, 4, "v_scale"));
@@ -550,8 +552,12 @@ static int check_decode_shape(const kfmi_decode_args *a) {
   if (a->S > 16) return fail(KFMI_EINVAL, "S must be at most 16 (got %lld)", (long long)a->S);
   if (a->B > 65535) return fail(KFMI_EINVAL, "B must be at most 65535 (got %lld)", (long long)a->B);
   if (a->max_pages < 1) return fail(KFMI_EINVAL, "max_pages must be >= 1 (got %lld)", (long long)a->max_pages);
-  if (a->page_size < 1 || a->max_pages > ((int64_t)1 << 31) / a->page_size)
-    return fail(KFMI_EINVAL, "a sequence's pages must hold at most 2^31 keys");
+  if (a->page_size < 1 || a->max_pages > ((int64_t)1 << 30) / a->page_size)
+    return fail(KFMI_EINVAL, "a sequence's pages must hold at most 2^30 keys");
+  // workgroups count the units of 128 keys, of all heads and blocks of 16 rows, in 32 bits
+  const int64_t rows = a->Hq / a->Hkv * a->S, units = (a->max_pages * a->page_size + 127) / 128;
+  if (a->B * a->Hkv * ((rows + 15) / 16) >= ((int64_t)1 << 31) / units)
+    return fail(KFMI_EINVAL, "B * Hkv * max_pages * page_size is too large");
   return KFMI_OK;
 }
 
@@ -590,8 +596,8 @@ int kfmi_cache_to_dense_bf16(const kfmi_cache_read_args *a, void *stream) {
   KFMI_TRY(check_index(a->lengths, a->index_flags, KFMI_I64_LENGTHS, "lengths"));
   KFMI_TRY(check_cache(a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->cache_stride, a->scale_stride, a->num_pages,
                        a->page_size, a->cache_type));
-  if (a->max_pages > ((int64_t)1 << 31) / a->page_size)
-    return fail(KFMI_EINVAL, "a sequence's pages must hold at most 2^31 keys");
+  if (a->max_pages > ((int64_t)1 << 30) / a->page_size)
+    return fail(KFMI_EINVAL, "a sequence's pages must hold at most 2^30 keys");
   KFMI_TRY(check_ptrs({{a->k, "k"}, {a->v, "v"}}));
   KFMI_TRY(check_device());
   return launch_status(kfmi::launch_cache_read(*a, (hipStream_t)stream), "cache read launch");

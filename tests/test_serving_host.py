@@ -135,7 +135,9 @@ REFUSED = [
     (WRITE, _write, dict(eps=-1.0), "eps"), (WRITE, _write, dict(eps=float("nan")), "eps"),
     (DECODE, _dec, dict(S=17), "at most 16"), (DECODE, _dec, dict(S=0), ">= 1"), (DECODE, _dec, dict(q=0), "q must not"),
     (DECODE, _dec, dict(Hq=9), "multiple of Hkv"), (DECODE, _dec, dict(max=0), "max_pages"),
-    (DECODE, _dec, dict(max=2 ** 40), "2^31 keys"), (DECODE, _dec, dict(B=70000), "65535"),
+    (DECODE, _dec, dict(B=65535, Hkv=64, Hq=64, max=2 ** 14), "too large"), (DECODE, _dec, dict(cs=(8192, 1024, 2 ** 24)), "tokens"),
+    (DECODE, _dec, dict(cs=(-8192, 1024, 128)), "cache strides"),
+    (DECODE, _dec, dict(max=2 ** 40), "2^30 keys"), (DECODE, _dec, dict(B=70000), "65535"),
     (DECODE, _dec, dict(flags=16), "index_flags"), (DECODE, _dec, dict(pages=0), "pages must not"),
     (DECODE, _dec, dict(lengths=P + 4, flags=8), "lengths must be 8"), (DECODE, _dec, dict(scale=0.0), "scale"),
     (DECODE, _dec, dict(cap=-1.0), "softcap"), (DECODE, _dec, dict(cap=float("nan")), "softcap"),
@@ -144,7 +146,7 @@ REFUSED = [
     (DECODE, _dec, dict(qs=(1, 8, 8)), "q strides"), (DECODE, _dec, dict(num=2 ** 62), "too many"),
     (READ, _read, dict(L=0), ">= 1"), (READ, _read, dict(L=2 ** 31), "2^31"), (READ, _read, dict(k=0), "k must not"),
     (READ, _read, dict(pages=P + 2), "pages must be 4"), (READ, _read, dict(B=65536), "65535"),
-    (READ, _read, dict(max=2 ** 31), "2^31 keys"),
+    (READ, _read, dict(max=2 ** 31), "2^30 keys"),
     (LOGPROBS, _lp, dict(v=0), ">= 1"), (LOGPROBS, _lp, dict(v=2 ** 31), "2^31"), (LOGPROBS, _lp, dict(n1=2 ** 26), "2^25"),
     (LOGPROBS, _lp, dict(top=33), "top must"), (LOGPROBS, _lp, dict(top=-1), "top must"),
     (LOGPROBS, _lp, dict(v=2), "top must"), (LOGPROBS, _lp, dict(kind=3), "logits_type"),
