@@ -19,6 +19,16 @@ __device__ __forceinline__ int64_t load_index(const void *p, bool wide, int64_t 
   return wide ? reinterpret_cast<const int64_t *>(p)[i] : (int64_t) reinterpret_cast<const int32_t *>(p)[i];
 }
 
+// The same in two words (low, high) through the constant address space: a wave-uniform
+// index becomes scalar loads, which do not wait for the vector loads in
+// flight.  For memory that nothing writes while the kernel runs.
+typedef const __attribute__((address_space(4))) int32_t const_i32_t;
+__device__ __forceinline__ int2 load_index_words(const void *p, bool wide, int64_t i) {
+  const_i32_t *w = (const_i32_t *)(reinterpret_cast<uintptr_t>(p));
+  const int lo = w[wide ? 2 * i : i], hi = w[wide ? 2 * i + 1 : i];
+  return int2{lo, wide ? hi : lo >> 31};
+}
+
 // E8M0: 2^(byte - 127), 255 is NaN.  2^-127 (byte 0) is a subnormal float.
 __device__ __forceinline__ float scale_value(uint32_t byte) {
   const uint32_t bits = byte << 23;

@@ -505,7 +505,7 @@ static int check_cache(const void *k, const void *v, const void *ks, const void 
   if (num_pages < 1) return fail(KFMI_EINVAL, "num_pages must be >= 1 (got %lld)", (long long)num_pages);
   if (page_size < 16 || page_size > (1 << 20) || (page_size & (page_size - 1)))
     return fail(KFMI_EINVAL, "page_size must be a power of two from 16 to 2^20 (got %lld)", (long long)page_size);
-  if (num_pages > ((int64_t)1 << 62) / page_size) return fail(KFMI_EINVAL, "too many pages");
+  if (num_pages >= (int64_t)1 << 31) return fail(KFMI_EINVAL, "num_pages must be below 2^31");
   KFMI_TRY(check_ptrs({{k, "k_cache"}, {v, "v_cache"}}));
   KFMI_TRY(check_strides(cs, 3, cache_type == KFMI_CACHE_E4M3 ? 16 : 8, "cache"));
   if (cs[2] >= (1 << 24)) return fail(KFMI_EINVAL, "the cache's stride between tokens must be below 2^24 elements");

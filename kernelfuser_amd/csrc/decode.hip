@@ -23,6 +23,7 @@
 //    crosses a border is joined, in order, by the workgroup that arrives last.
 #include <cstdio>
 #include <string>
+#include <type_traits>
 
 #include "cache_common.h"
 #include "kfmi_launch.h"
@@ -34,7 +35,6 @@ constexpr int WV = 4;            // waves per workgroup
 constexpr int NTHR = 64 * WV;
 constexpr int UNIT = 32 * WV;    // keys per unit of work
 constexpr int SC1 = 16;          // cache policy of agent-coherent accesses
-constexpr float LOG2E = 1.44269504088896340736f;
 
 struct DecodeParams {
   const uint16_t *q;
@@ -45,31 +45,62 @@ struct DecodeParams {
   int *counters;    // NULL: no workspace, no sequence is split
   float *partials;  // 2 slots per workgroup
   int64_t qs[3], cs[3], es[2];
-  int64_t pages_stride, lengths_stride, num_pages;
-  int B, hq, hk, S, group, rows, rblocks;  // rows = group * S, in blocks of 16 * NT
+  int64_t pages_stride, lengths_stride;
+  int num_pages, B, hq, hk, S, group, rows, rblocks;  // rows = group * S, in blocks of 16 * NT
   int capacity, window, min_units;
   int page_shift, page_mask;
   bool pages64, len64;
-  float scale, softcap;  // softcap 0: none
+  float score_scale;  // of q . k: to the exponent of 2 (cap 0), or to the argument 2 y log2(e) of the capped one
+  float cap;          // softcap * log2(e); 0: none
 };
 
 // What a launch reads of one sequence.
 struct Sequence {
   int len;    // 0 where the given one is wrong
-  int start;  // first key of the first unit: below every key that a query sees, a multiple of 32
+  int lo;     // first key that a query sees
+  int start;  // first key of the first unit: lo or below, a multiple of 32
   int units;
   bool bad;
 };
 
 __device__ __forceinline__ Sequence sequence(const DecodeParams &p, int b) {
   Sequence s;
-  const int64_t len = load_index(p.lengths, p.len64, (int64_t)b * p.lengths_stride);
-  s.bad = len < 0 || len > p.capacity;
-  s.len = s.bad ? 0 : (int)len;
-  const int lo = p.window > 0 ? max(0, s.len - p.S - p.window + 1) : 0;
-  s.start = lo & ~31;
-  s.units = max(1, (s.len - s.start + UNIT - 1) / UNIT);
+  const int2 len = load_index_words(p.lengths, p.len64, (int64_t)b * p.lengths_stride);
+  s.bad = len.y != 0 || (uint32_t)len.x > (uint32_t)p.capacity;
+  s.len = s.bad ? 0 : len.x;
+  s.lo = p.window > 0 ? max(0, s.len - p.S - p.window + 1) : 0;
+  s.start = s.lo & ~31;
+  s.units = p.counters ? max(1, (s.len - s.start + UNIT - 1) / UNIT) : 1;  // never split: one unit of all keys
   return s;
+}
+
+// A workgroup's part of one sequence, head and block of rows: units k0 .. k1 - 1.
+struct Item {
+  Sequence s;
+  int b, h, rb;
+  uint32_t k0, k1;
+  int key0, key1;
+};
+
+__device__ __forceinline__ Item item_at(const DecodeParams &p, int b, uint32_t rem, uint32_t left) {
+  Item it;
+  it.s = sequence(p, b);
+  it.b = b;
+  const uint32_t units = (uint32_t)it.s.units, item = rem / units;
+  it.k0 = rem - item * units;
+  it.k1 = min(units, it.k0 + left);
+  it.h = (int)(item / (uint32_t)p.rblocks);
+  it.rb = (int)(item % (uint32_t)p.rblocks);
+  it.key0 = it.s.start + (int)it.k0 * UNIT;
+  it.key1 = p.counters ? min(it.s.len, it.s.start + (int)it.k1 * UNIT) : it.s.len;
+  return it;
+}
+
+// x, of which the compiler knows nothing: what is computed from it stays where it
+// is used, instead of in registers across the whole of the kernel's loop.
+__device__ __forceinline__ int opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
 }
 
 __device__ __forceinline__ float max_rows4(float x) {  // over lanes l, l^16, l^32, l^48
@@ -136,199 +167,219 @@ struct VTile {
   }
 };
 
+// Waves per SIMD that the registers of a step (K, V, Q, the accumulators) leave room for.
+constexpr int waves_per_simd(int d, bool fp8, int nt) { return d * nt * (fp8 ? 1 : d / 128) <= 256 ? 2 : 1; }
+
 // MULTI: S > 1.
 template <int D, bool FP8, int NT, bool MULTI>
-__global__ __launch_bounds__(NTHR, NT * D <= 256 ? 2 : 1) void decode_kernel(DecodeParams p) {
+__global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kernel(DecodeParams p) {
   constexpr int NK = D / 32;    // matrix steps of q . k
   constexpr int ND = D / 16;    // products of P V
   constexpr int NX = ND / 8;
   constexpr int ES = FP8 ? 1 : 2;
   constexpr int ROWS = 16 * NT;
   constexpr int SLOT = ROWS * (D + 2);  // floats: O row by row, then (m, l) of each row
-  constexpr int LDX = 36;               // floats per row of the exchange (32 and padding)
+  constexpr int LDX = D + 4;            // floats per row of the exchange
   constexpr int MG = NTHR / (D / 8);    // groups of the join
   constexpr int EX = WV * ROWS * LDX > MG * 4 * D ? WV * ROWS * LDX : MG * 4 * D;
   __shared__ __attribute__((aligned(16))) float ex[EX];
   __shared__ float ml[(WV * ROWS > MG * 4 ? WV * ROWS : MG * 4) * 2];
-  __shared__ uint32_t plan[WV + 3];
+  __shared__ uint32_t arrived;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, c = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const bool split = p.counters != nullptr;
   const uint32_t ipb = (uint32_t)(p.hk * p.rblocks);  // items (head, block of rows) per sequence
 
-  // This workgroup's share [g0, g1) of all units: sequences in the order
-  // 0, NTHR, 2 NTHR, .., 1, NTHR + 1, .. (thread by thread).
+  // This workgroup's share [g0, g1) of all units, the sequences in the order
+  // 0, 64, 128, .., 1, 65, .. (lane by lane); every wave finds it by itself.
   uint32_t mine = 0;
-  for (int b = tid; b < p.B; b += NTHR) mine += (split ? (uint32_t)sequence(p, b).units : 1u) * ipb;
+  for (int b = lane; b < p.B; b += 64) mine += (uint32_t)sequence(p, b).units * ipb;
   uint32_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const uint32_t y = (uint32_t)__shfl_up((int)incl, o);
     if (lane >= o) incl += y;
   }
-  if (lane == 63) plan[w] = incl;
-  __syncthreads();
-  uint32_t total = 0, before = 0;
-#pragma unroll
-  for (int i = 0; i < WV; ++i) {
-    if (i < w) before += plan[i];
-    total += plan[i];
-  }
-  incl += before;
+  const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
   const uint32_t per = max((total + gridDim.x - 1) / gridDim.x, (uint32_t)p.min_units);
   const uint32_t g0 = blockIdx.x * per, g1 = min(g0 + per, total);
   if (g0 >= total) return;  // workgroup-uniform
-  if (incl - mine <= g0 && g0 < incl) {
-    uint32_t rem = g0 - (incl - mine);
-    int b = tid;
-    for (;;) {
-      const uint32_t u = (split ? (uint32_t)sequence(p, b).units : 1u) * ipb;
-      if (rem < u) break;
-      rem -= u;
-      b += NTHR;
-    }
-    plan[WV] = (uint32_t)b;
-    plan[WV + 1] = rem;
+  int b = __builtin_ctzll(__ballot(incl > g0));
+  uint32_t rem = g0 - (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), b);
+  for (;;) {
+    const uint32_t u = (uint32_t)sequence(p, b).units * ipb;
+    if (rem < u) break;
+    rem -= u;
+    b += 64;
   }
-  __syncthreads();
-  int b = __builtin_amdgcn_readfirstlane((int)plan[WV]);
-  uint32_t rem = (uint32_t)__builtin_amdgcn_readfirstlane((int)plan[WV + 1]);
 
-  for (uint32_t g = g0; g < g1;) {
-    const Sequence s = sequence(p, b);
-    const uint32_t units = split ? (uint32_t)s.units : 1u;
-    const uint32_t item = rem / units, k0 = rem - item * units;
-    const uint32_t k1 = min(units, k0 + (g1 - g));
-    const int h = (int)(item / (uint32_t)p.rblocks), rb = (int)(item % (uint32_t)p.rblocks);
-    const int key0 = s.start + (int)k0 * UNIT;
-    const int key1 = split ? min(s.len, s.start + (int)k1 * UNIT) : s.len;
-    const int seq_lo = p.window > 0 ? max(0, s.len - p.S - p.window + 1) : 0;
-    // keys that every query sees: [all_lo, all_hi)
-    const int all_hi = s.len - p.S + 1, all_lo = p.window > 0 ? max(0, s.len - p.window) : 0;
-
-    int hi[NT], lo[NT], token[NT];
-    u32x4_t qf[NT][NK];
+  // The pages of the two groups of 16 keys from j on.  A group that no query
+  // sees takes the nearest page that one does: its own entry may be anything.
+  int2 pg[2];
+  auto request_pages = [&](const Item &it, int j0) {
+    const int64_t row0 = (int64_t)it.b * p.pages_stride;
+    const int lo = it.s.lo >> p.page_shift, hi = max(it.s.len - 1, 0) >> p.page_shift;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int r = rb * ROWS + 16 * t + n;
-      const bool live = r < p.rows;
-      const int rr = live ? r : 0;
-      const int gi = rr / p.S;
-      token[t] = rr - gi * p.S;
-      hi[t] = live ? s.len - p.S + token[t] + 1 : 0;
-      lo[t] = p.window > 0 ? max(0, hi[t] - p.window) : 0;
-      const uint16_t *src = p.q + b * p.qs[0] + (int64_t)(h * p.group + gi) * p.qs[1] + token[t] * p.qs[2];
+    for (int t = 0; t < 2; ++t)
+      pg[t] = load_index_words(p.pages, p.pages64, row0 + min(max((j0 + 16 * t) >> p.page_shift, lo), hi));
+  };
+  const uint32_t row = (uint32_t)p.cs[2] * ES;  // bytes from token to token
+  const char *kb[2], *vb[2];
+  const uint8_t *ksb[2], *vsb[2];
+  auto look_up = [&](const Item &it, int j0, bool &bad) {
 #pragma unroll
-      for (int k = 0; k < NK; ++k) {
-        const int d = FP8 ? 64 * (k / 2) + 16 * c + 8 * (k & 1) : 32 * k + 8 * c;
-        qf[t][k] = ld16(src + d);
+    for (int t = 0; t < 2; ++t) {
+      const bool wrong = pg[t].y != 0 || (uint32_t)pg[t].x >= (uint32_t)p.num_pages;
+      bad |= wrong;
+      const int64_t page = wrong ? 0 : pg[t].x;
+      const int64_t at = (j0 + 16 * t) & p.page_mask;
+      const int64_t off = (page * p.cs[0] + it.h * p.cs[1] + at * p.cs[2]) * ES;
+      kb[t] = p.k_cache + off;
+      vb[t] = p.v_cache + off;
+      if constexpr (FP8) {
+        const int64_t so = page * p.es[0] + it.h * p.es[1] + at;
+        ksb[t] = p.k_scale + so;
+        vsb[t] = p.v_scale + so;
       }
     }
+  };
+  u32x4_t qf[NT][NK];
+  auto load_q = [&](const Item &it) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int r = it.rb * ROWS + 16 * t + opaque(n), rr = r < p.rows ? r : 0, gi = rr / p.S;
+      const uint16_t *src = p.q + it.b * p.qs[0] + (int64_t)(it.h * p.group + gi) * p.qs[1] + (rr - gi * p.S) * p.qs[2];
+#pragma unroll
+      for (int k = 0; k < NK; ++k)
+        qf[t][k] = ld16(src + (FP8 ? 64 * (k / 2) + 16 * c + 8 * (k & 1) : 32 * k + 8 * c));
+    }
+  };
+  u32x4_t kw[2][FP8 ? NK / 2 : NK];
+  uint32_t ksw[2], vsw[2];
+  VTile<D, FP8> v;
+  auto load_k = [&]() {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int k = 0; k < (FP8 ? NK / 2 : NK); ++k)
+        kw[t][k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(kb[t] + (n * row + 16 * c + 64 * k)));
+      if constexpr (FP8) ksw[t] = *reinterpret_cast<const uint32_t *>(ksb[t] + 4 * c);
+    }
+  };
+  auto load_v = [&]() {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const char *src = vb[j / 4] + (4 * c + (j & 3)) * row;
+      if constexpr (FP8 && D == 128) {
+        const u32x2_t x = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t *>(src + 8 * n));
+        v.w[j][0] = x[0];
+        v.w[j][1] = x[1];
+      } else {
+#pragma unroll
+        for (int x = 0; x < VTile<D, FP8>::W / 4; ++x) {
+          const u32x4_t y = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(src + 16 * n + 256 * x));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v.w[j][4 * x + e] = y[e];
+        }
+      }
+    }
+    if constexpr (FP8) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) vsw[t] = *reinterpret_cast<const uint32_t *>(vsb[t] + 4 * c);
+    }
+  };
+
+  // The item's first step of this wave: whether there is one, and its loads.
+  auto begin = [&](const Item &it, bool &bad) {
+    load_q(it);
+    const int j0 = it.key0 + 32 * w;
+    if (j0 >= it.key1) return false;
+    request_pages(it, j0);
+    look_up(it, j0, bad);
+    load_k();
+    load_v();
+    request_pages(it, j0 + UNIT);
+    return true;
+  };
+
+  uint32_t g = g0;
+  Item it = item_at(p, b, rem, g1 - g);
+  bool bad = it.s.bad, some = begin(it, bad);
+  for (;;) {
+    const Sequence s = it.s;
+    // keys that every query sees: [all_lo, all_hi)
+    const int all_hi = s.len - p.S + 1, all_lo = p.window > 0 ? max(0, s.len - p.window) : 0;
+    int hi[NT], lo[NT];
     f32x4_t acc[NT][ND];
     float m[NT], l[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
+      const int r = it.rb * ROWS + 16 * t + opaque(n);
+      hi[t] = r < p.rows ? s.len - p.S + r % p.S + 1 : 0;
+      lo[t] = p.window > 0 ? max(0, hi[t] - p.window) : 0;
       m[t] = -INFINITY;
       l[t] = 0.f;
 #pragma unroll
       for (int d = 0; d < ND; ++d) acc[t][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
-    bool bad = s.bad;
-
-    for (int j0 = key0 + 32 * w; j0 < key1; j0 += UNIT) {
-      // pages of the two groups of 16 keys; a group that no query sees is not looked up
-      const char *kb[2], *vb[2];
-      const uint8_t *ksb[2], *vsb[2];
+    if (some) {
+      // Q is waited for here, once: in the loop the wait would be one for the
+      // youngest loads, K and V of the next step.
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int j = j0 + 16 * t;
-        const bool seen = j < s.len && j + 16 > seq_lo;
-        int64_t page = 0;
-        if (seen) page = load_index(p.pages, p.pages64, (int64_t)b * p.pages_stride + (j >> p.page_shift));
-        if (page < 0 || page >= p.num_pages) {
-          bad = true;
-          page = 0;
-        }
-        const int64_t at = j & p.page_mask;
-        const int64_t off = (page * p.cs[0] + h * p.cs[1] + at * p.cs[2]) * ES;
-        kb[t] = p.k_cache + off;
-        vb[t] = p.v_cache + off;
-        if constexpr (FP8) {
-          const int64_t so = page * p.es[0] + h * p.es[1] + at;
-          ksb[t] = p.k_scale + so;
-          vsb[t] = p.v_scale + so;
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int k = 0; k < NK; ++k) asm volatile("" ::"v"(qf[t][k]));
+      // K of the next step is requested as soon as this step's K has been used,
+      // V likewise; the last step has none to request.
+      int j0 = it.key0 + 32 * w;
+      auto step = [&](auto more) {
+      if constexpr (more.value) {
+        look_up(it, j0 + UNIT, bad);
+        request_pages(it, j0 + 2 * UNIT);
+      }
+      const bool edge = j0 < all_lo || j0 + 32 > all_hi;  // wave-uniform
+      f32x4_t z[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) z[t][0] = z[t][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+          u32x4_t a;
+          if constexpr (FP8) {
+            const uint32_t x0 = kw[u][k / 2][2 * (k & 1)], x1 = kw[u][k / 2][2 * (k & 1) + 1];
+            a = u32x4_t{bf16_of_e4m3(x0, false), bf16_of_e4m3(x0, true), bf16_of_e4m3(x1, false), bf16_of_e4m3(x1, true)};
+          } else {
+            a = kw[u][k];
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) z[t][u] = mfma(a, qf[t][k], z[t][u]);
         }
       }
-      const uint32_t row = (uint32_t)p.cs[2] * ES;  // bytes from token to token
-      u32x4_t kw[2][FP8 ? NK / 2 : NK];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int k = 0; k < (FP8 ? NK / 2 : NK); ++k)
-          kw[t][k] = *reinterpret_cast<const u32x4_t *>(kb[t] + (n * row + 16 * c + 64 * k));
-      uint32_t ksw[2], vsw[2];
+      float ks[FP8 ? 8 : 1], vs[FP8 ? 8 : 1];
       if constexpr (FP8) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          ksw[t] = *reinterpret_cast<const uint32_t *>(ksb[t] + 4 * c);
-          vsw[t] = *reinterpret_cast<const uint32_t *>(vsb[t] + 4 * c);
+        for (int i = 0; i < 8; ++i) {
+          ks[i] = p.score_scale * scale_value((ksw[i / 4] >> (8 * (i & 3))) & 255u);
+          vs[i] = scale_value((vsw[i / 4] >> (8 * (i & 3))) & 255u);
+          const int j = j0 + 16 * (i / 4) + 4 * c + (i & 3);
+          if (edge && (j < s.lo || j >= s.len)) ks[i] = vs[i] = 0.f;  // one that is not seen may be NaN
         }
       }
-      VTile<D, FP8> v;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const char *src = vb[j / 4] + (4 * c + (j & 3)) * row;
-        if constexpr (FP8 && D == 128) {
-          const u32x2_t x = *reinterpret_cast<const u32x2_t *>(src + 8 * n);
-          v.w[j][0] = x[0];
-          v.w[j][1] = x[1];
-        } else {
-#pragma unroll
-          for (int x = 0; x < VTile<D, FP8>::W / 4; ++x) {
-            const u32x4_t y = *reinterpret_cast<const u32x4_t *>(src + 16 * n + 256 * x);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v.w[j][4 * x + e] = y[e];
-          }
-        }
-      }
-
-      const bool edge = j0 < all_lo || j0 + 32 > all_hi;  // wave-uniform
+      __builtin_amdgcn_sched_barrier(0);  // the loads take the registers of what they follow
+      if constexpr (more.value) load_k();
+      __builtin_amdgcn_sched_barrier(0);
       u32x4_t ph[NT], pl[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float sc[8];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          f32x4_t z = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 8; ++i) sc[i] = z[t][i / 4][i & 3] * (FP8 ? ks[i] : p.score_scale);
+        if (p.cap > 0.f) {
+          // cap * tanh(x / cap) with tanh y = 1 - 2 / (e^2y + 1); the score is 2 y log2(e) here
 #pragma unroll
-          for (int k = 0; k < NK; ++k) {
-            u32x4_t a;
-            if constexpr (FP8) {
-              const uint32_t x0 = kw[u][k / 2][2 * (k & 1)], x1 = kw[u][k / 2][2 * (k & 1) + 1];
-              a = u32x4_t{bf16_of_e4m3(x0, false), bf16_of_e4m3(x0, true), bf16_of_e4m3(x1, false), bf16_of_e4m3(x1, true)};
-            } else {
-              a = kw[u][k];
-            }
-            z = mfma(a, qf[t][k], z);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float x = z[i] * p.scale;
-            if constexpr (FP8) x *= scale_value((ksw[u] >> (8 * i)) & 255u);
-            sc[4 * u + i] = x;
-          }
+          for (int i = 0; i < 8; ++i)
+            sc[i] = fmaf(-2.0f * p.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(sc[i]) + 1.0f), p.cap);
         }
-        if (p.softcap > 0.f) {
-          // cap * tanh(x / cap), tanh y = 1 - 2 / (e^2y + 1)
-          const float a = 2.0f * LOG2E / p.softcap, cap = p.softcap;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float e = __builtin_amdgcn_exp2f(sc[i] * a);
-            sc[i] = fmaf(-2.0f * cap, __builtin_amdgcn_rcpf(e + 1.0f), cap);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sc[i] *= LOG2E;
         if (edge) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -354,16 +405,14 @@ __global__ __launch_bounds__(NTHR, NT * D <= 256 ? 2 : 1) void decode_kernel(Dec
         for (int i = 0; i < 8; ++i) {
           pr[i] = __builtin_amdgcn_exp2f(sc[i] - base);
           sum += pr[i];
+          if constexpr (FP8) pr[i] *= vs[i];
+        }
+        if (FP8 && MULTI && edge) {  // a scale that this query does not see may be NaN
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (sc[i] == -INFINITY) pr[i] = 0.f;
         }
         l[t] += sum;
-        if constexpr (FP8) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float x = pr[i] * scale_value((vsw[i / 4] >> (8 * (i & 3))) & 255u);
-            const int j = j0 + 16 * (i / 4) + 4 * c + (i & 3);
-            pr[i] = edge && (j < lo[t] || j >= hi[t]) ? 0.f : x;  // a scale that is not seen may be NaN
-          }
-        }
         // p = hi + lo, both bf16 and both positive where p is: lo keeps 2^-7
         // to 2^-6 of p, so that an infinite v, which meets both, stays an infinity.
         float lo_[8];
@@ -384,7 +433,7 @@ __global__ __launch_bounds__(NTHR, NT * D <= 256 ? 2 : 1) void decode_kernel(Dec
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int key = j0 + 16 * (j / 4) + 4 * c + (j & 3);
-          bool drop = key < seq_lo || key >= s.len;
+          bool drop = key < s.lo || key >= s.len;
           if constexpr (MULTI) {
             // A value that is not finite, of a key that only some of the queries
             // see, would reach the others as 0 * NaN: the key is taken out, and the
@@ -409,96 +458,122 @@ __global__ __launch_bounds__(NTHR, NT * D <= 256 ? 2 : 1) void decode_kernel(Dec
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[t][d] = mfma(a, pl[t], mfma(a, ph[t], acc[t][d]));
       }
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (more.value) load_v();
+      __builtin_amdgcn_sched_barrier(0);
+      };
+      for (; j0 + UNIT < it.key1; j0 += UNIT) step(std::true_type{});
+      step(std::false_type{});
     }
 
-    // Join the waves: maxima and sums first, then O in pieces of 32 columns.
-    const bool any_bad = __syncthreads_or(bad);
+    // The next item's first loads run while this one is written.
+    const uint32_t istart = g - it.k0;
+    const uint32_t w0 = istart / per, w1 = (istart + (uint32_t)s.units - 1) / per;  // the workgroups that share the item
+    g += it.k1 - it.k0;
+    rem += it.k1 - it.k0;
+    if (rem == (uint32_t)s.units * ipb) {
+      rem = 0;
+      b += 64;
+      if (b >= p.B) b = b % 64 + 1;
+    }
+    const bool again = g < g1;
+    Item next = it;
+    bool next_bad = false, next_some = false;
+    if (again) {
+      next = item_at(p, b, rem, g1 - g);
+      next_bad = next.s.bad;
+      next_some = begin(next, next_bad);
+    }
+
+    // Join the waves: maxima, sums and O of the rows in use through LDS.
+    const bool whole = w0 == w1;
+    const int rows_here = min(ROWS, p.rows - it.rb * ROWS);
+    const int xtid = opaque(tid), xn = xtid & 15, xc = (xtid & 63) >> 4;
+    const int64_t out0 = ((int64_t)(it.b * p.hq + it.h * p.group) * p.S + it.rb * ROWS) * D;
+    float *slot = p.partials + (int64_t)(2 * blockIdx.x + (w0 == blockIdx.x ? 1 : 0)) * SLOT;
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc(whole ? p.partials : slot, 0, whole ? 0 : SLOT * 4, 0x00020000);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const float sum = sum_rows4(l[t]);
-      if (c == 0) {
-        ml[(w * ROWS + 16 * t + n) * 2] = m[t];
-        ml[(w * ROWS + 16 * t + n) * 2 + 1] = sum;
+      if (16 * t + xn < rows_here) {
+        float *dst = ex + (w * ROWS + 16 * t + xn) * LDX;
+        if (xc == 0) {
+          ml[(w * ROWS + 16 * t + xn) * 2] = m[t];
+          ml[(w * ROWS + 16 * t + xn) * 2 + 1] = sum;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int x = 0; x < NX; ++x) {
+            float *o = dst + d_of<D, FP8>(4 * xc + i, x);
+#pragma unroll
+            for (int e = 0; e < 8; e += 4)
+              *reinterpret_cast<f32x4_t *>(o + e) =
+                  f32x4_t{acc[t][8 * x + e][i], acc[t][8 * x + e + 1][i], acc[t][8 * x + e + 2][i], acc[t][8 * x + e + 3][i]};
+          }
       }
     }
-    const uint32_t istart = g - k0;
-    const uint32_t w0 = istart / per, w1 = split ? (istart + units - 1) / per : w0;
-    const bool whole = w0 == w1;
-    const int rows_here = min(ROWS, p.rows - rb * ROWS);
-    const int64_t out0 = ((int64_t)(b * p.hq + h * p.group) * p.S + rb * ROWS) * D;
-    float *slot = nullptr;
-    __amdgpu_buffer_rsrc_t rs;
-    if (!whole) {
-      slot = p.partials + (int64_t)(2 * blockIdx.x + (w0 == blockIdx.x ? 1 : 0)) * SLOT;
-      rs = __builtin_amdgcn_make_buffer_rsrc(slot, 0, SLOT * 4, 0x00020000);
-    }
+    const bool any_bad = __syncthreads_or(bad);
+    const float nan = __uint_as_float(0x7fc00000u);
+    for (int piece = xtid; piece < rows_here * (D / 4); piece += NTHR) {
+      const int r = piece / (D / 4), d = piece % (D / 4) * 4;
+      float mm[WV], ll[WV], top = -INFINITY;
+      f32x4_t o[WV];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+      for (int y = 0; y < WV; ++y) {
+        mm[y] = ml[(y * ROWS + r) * 2];
+        ll[y] = ml[(y * ROWS + r) * 2 + 1];
+        o[y] = *reinterpret_cast<const f32x4_t *>(ex + (y * ROWS + r) * LDX + d);
+      }
 #pragma unroll
-      for (int x = 0; x < NX; ++x) {
-        __syncthreads();
+      for (int y = 0; y < WV; ++y) top = fmaxf(top, mm[y]);
+      const float base = top == -INFINITY ? 0.f : top;
+      f32x4_t sum4 = {0.f, 0.f, 0.f, 0.f};
+      float sum = 0.f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          float *dst = ex + (w * ROWS + 16 * t + n) * LDX + 8 * c;
+      for (int y = 0; y < WV; ++y) {
+        const float a = __builtin_amdgcn_exp2f(mm[y] - base);
+        sum = fmaf(a, ll[y], sum);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) dst[e] = acc[t][8 * x + e][i];
-        }
-        __syncthreads();
-        for (int piece = tid; piece < 4 * rows_here; piece += NTHR) {
-          const int r = piece >> 2, cc = piece & 3;
-          float mm = -INFINITY;
+        for (int e = 0; e < 4; ++e) sum4[e] = fmaf(a, o[y][e], sum4[e]);
+      }
+      if (whole) {
+        const bool none = s.len - p.S + (it.rb * ROWS + r) % p.S < 0;  // no key at all
+        float y[4];
 #pragma unroll
-          for (int y = 0; y < WV; ++y) mm = fmaxf(mm, ml[(y * ROWS + r) * 2]);
-          const float base = mm == -INFINITY ? 0.f : mm;
-          float o[8] = {}, sum = 0.f;
-#pragma unroll
-          for (int y = 0; y < WV; ++y) {
-            const float a = __builtin_amdgcn_exp2f(ml[(y * ROWS + r) * 2] - base);
-            sum = fmaf(a, ml[(y * ROWS + r) * 2 + 1], sum);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = fmaf(a, ex[(y * ROWS + r) * LDX + 8 * cc + e], o[e]);
-          }
-          const int d = d_of<D, FP8>(4 * cc + i, x);
-          if (whole) {
-            const int tk = (rb * ROWS + r) % p.S;
-            const bool none = s.len - p.S + tk < 0;  // no key at all
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              y[e] = any_bad ? __uint_as_float(0x7fc00000u) : none ? 0.f : o[e] / sum;
-            st16(p.out + out0 + (int64_t)r * D + d, pack8(y));
-          } else {
-            __builtin_amdgcn_raw_buffer_store_b128(
-                __builtin_bit_cast(u32x4_t, f32x4_t{o[0], o[1], o[2], o[3]}), rs, (r * D + d) * 4, 0, SC1);
-            __builtin_amdgcn_raw_buffer_store_b128(
-                __builtin_bit_cast(u32x4_t, f32x4_t{o[4], o[5], o[6], o[7]}), rs, (r * D + d + 4) * 4, 0, SC1);
-            if (i == 0 && x == 0 && cc == 0) {
-              // a wrong page is handed on as a sum that is NaN
-              const float su = any_bad ? __uint_as_float(0x7fc00000u) : sum;
-              __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(mm), __float_as_uint(su)}, rs,
-                                                    (ROWS * D + 2 * r) * 4, 0, SC1);
-            }
-          }
-        }
+        for (int e = 0; e < 4; ++e) y[e] = any_bad ? nan : none ? 0.f : sum4[e] / sum;
+        *reinterpret_cast<u32x2_t *>(p.out + out0 + (int64_t)r * D + d) =
+            u32x2_t{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+      } else {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, sum4), rs, (r * D + d) * 4, 0, SC1);
+        if (d == 0)  // a wrong page is handed on as a sum that is NaN
+          __builtin_amdgcn_raw_buffer_store_b64(u32x2_t{__float_as_uint(top), __float_as_uint(any_bad ? nan : sum)}, rs,
+                                                (ROWS * D + 2 * r) * 4, 0, SC1);
       }
     }
     if (!whole) {
-      // Every store of this thread has completed, then one arrival per
-      // workgroup (release before, acquire after, at agent scope).
+      // The parts are written and read with agent-coherent accesses (SC1), which
+      // pass the caches of an XCD by: a store that has completed (vmcnt) is what
+      // any later SC1 load gets.  So the arrival needs no L2 writeback or
+      // invalidation (release and acquire fences cost 18 us a launch here).
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      if (tid == 0) {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
-        plan[WV + 2] = (uint32_t)atomicAdd(p.counters + w0, 1);
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-      }
+      if (tid == 0)
+        arrived = (uint32_t)__hip_atomic_fetch_add(p.counters + w0, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       __syncthreads();
-      if (plan[WV + 2] == w1 - w0) {  // the last: join the parts w0 .. w1 in order
-        const int piece = tid % (D / 8), grp = tid / (D / 8);
+      if (arrived == w1 - w0) {  // the last: join the parts w0 .. w1 in order
+        // A thread sums 8 columns of 4 rows over every pgs-th part; the groups of threads
+        // that the parts leave over take other rows.
+        const int tid_ = opaque(tid);
         const uint32_t parts = w1 - w0 + 1;
+        const int piece = tid_ % (D / 8), grp = tid_ / (D / 8);
+        int pgs = 1;
+        while (pgs < MG && (uint32_t)pgs < parts) pgs *= 2;
+        const int pgi = grp % pgs, step = 4 * (MG / pgs);
         const auto all = __builtin_amdgcn_make_buffer_rsrc(p.partials, 0, 2 * gridDim.x * (SLOT * 4), 0x00020000);
 #pragma unroll 1
-        for (int r0 = 0; r0 < rows_here; r0 += 4) {
+        for (int rb0 = 0; rb0 < rows_here; rb0 += step) {
+          const int r0 = rb0 + grp / pgs * 4;
           float o[4][8] = {}, mm[4], sum[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -506,7 +581,7 @@ __global__ __launch_bounds__(NTHR, NT * D <= 256 ? 2 : 1) void decode_kernel(Dec
             sum[r] = 0.f;
           }
 #pragma unroll 1
-          for (uint32_t k = grp; k < parts; k += MG) {
+          for (uint32_t k = pgi; k < parts; k += pgs) {
             const uint32_t from = w0 + k;
             const uint32_t at = (2 * from + (from == w0 ? 1 : 0)) * (SLOT * 4);
             u32x4_t po[4][2];
@@ -538,42 +613,43 @@ __global__ __launch_bounds__(NTHR, NT * D <= 256 ? 2 : 1) void decode_kernel(Dec
               ml[(grp * 4 + r) * 2 + 1] = sum[r];
             }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ex[(grp * 4 + r) * D + 8 * piece + e] = o[r][e];
+            for (int e = 0; e < 8; e += 4)
+              *reinterpret_cast<f32x4_t *>(ex + (grp * 4 + r) * D + 8 * piece + e) =
+                  f32x4_t{o[r][e], o[r][e + 1], o[r][e + 2], o[r][e + 3]};
           }
           __syncthreads();
-          for (int k = tid; k < 4 * (D / 8); k += NTHR) {
-            const int r = k / (D / 8), pc = k % (D / 8);
-            if (r0 + r >= rows_here) continue;
+          for (int k = tid_; k < step * (D / 4); k += NTHR) {
+            const int rr = k / (D / 4), d = k % (D / 4) * 4;
+            const int r = rb0 + rr, g4 = rr / 4 * pgs, r4 = rr % 4;
+            if (r >= rows_here) continue;
             float top = -INFINITY;
-#pragma unroll
-            for (int y = 0; y < MG; ++y) top = fmaxf(top, ml[(y * 4 + r) * 2]);
+#pragma unroll 4
+            for (int y = 0; y < pgs; ++y) top = fmaxf(top, ml[((g4 + y) * 4 + r4) * 2]);
             const float base = top == -INFINITY ? 0.f : top;
-            float y8[8] = {}, su = 0.f;
+            f32x4_t y4 = {0.f, 0.f, 0.f, 0.f};
+            float su = 0.f;
+#pragma unroll 4
+            for (int y = 0; y < pgs; ++y) {
+              const int at = (g4 + y) * 4 + r4;
+              const float a = __builtin_amdgcn_exp2f(ml[at * 2] - base);
+              const f32x4_t v4 = *reinterpret_cast<const f32x4_t *>(ex + at * D + d);
+              su = fmaf(a, ml[at * 2 + 1], su);
 #pragma unroll
-            for (int y = 0; y < MG; ++y) {
-              const float a = __builtin_amdgcn_exp2f(ml[(y * 4 + r) * 2] - base);
-              su = fmaf(a, ml[(y * 4 + r) * 2 + 1], su);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) y8[e] = fmaf(a, ex[(y * 4 + r) * D + 8 * pc + e], y8[e]);
+              for (int e = 0; e < 4; ++e) y4[e] = fmaf(a, v4[e], y4[e]);
             }
-            const int tk = (rb * ROWS + r0 + r) % p.S;
-            const bool none = s.len - p.S + tk < 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y8[e] = none && su == su ? 0.f : y8[e] / su;
-            st16(p.out + out0 + (int64_t)(r0 + r) * D + 8 * pc, pack8(y8));
+            *reinterpret_cast<u32x2_t *>(p.out + out0 + (int64_t)r * D + d) =
+                u32x2_t{pack_bf16x2(y4[0] / su, y4[1] / su), pack_bf16x2(y4[2] / su, y4[3] / su)};
           }
+          __syncthreads();
         }
-        if (tid == 0) atomicExch(p.counters + w0, 0);
+        if (tid == 0) __hip_atomic_store(p.counters + w0, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
     }
+    if (!again) break;
     __syncthreads();  // the exchange's memory is free again
-    g += k1 - k0;
-    rem += k1 - k0;
-    if (rem == units * ipb) {
-      rem = 0;
-      b += NTHR;
-      if (b >= p.B) b = b % NTHR + 1;
-    }
+    it = next;
+    bad = next_bad;
+    some = next_some;
   }
 }
 
@@ -590,7 +666,7 @@ Plan plan_of(const kfmi_decode_args &a) {
   r.nt = rows <= 16 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
   r.rblocks = (int)((rows + 16 * r.nt - 1) / (16 * r.nt));
   const int64_t units = a.B * a.Hkv * r.rblocks * ((a.max_pages * a.page_size + UNIT - 1) / UNIT);
-  const int64_t round = r.nt * a.D <= 256 ? 512 : 256;  // workgroups that run at once: two or one per CU
+  const int64_t round = 256 * waves_per_simd((int)a.D, a.cache_type == KFMI_CACHE_E4M3, r.nt);  // workgroups that run at once: two or one per CU
   r.grid = units < round ? units : round;
   r.slot_floats = 16 * r.nt * (a.D + 2);
   return r;
@@ -643,7 +719,7 @@ hipError_t launch_decode(const kfmi_decode_args &a, hipStream_t stream) {
   }
   for (int i = 0; i < 2; ++i) p.es[i] = a.scale_stride[i];
   p.pages_stride = a.pages_stride; p.lengths_stride = a.lengths_stride;
-  p.num_pages = a.num_pages;
+  p.num_pages = (int)a.num_pages;
   p.capacity = (int)(a.max_pages * a.page_size);
   p.window = (int)(a.window < p.capacity ? a.window : 0);  // a window of all keys is none
   p.min_units = 1;
@@ -655,8 +731,9 @@ hipError_t launch_decode(const kfmi_decode_args &a, hipStream_t stream) {
   p.page_mask = (int)(a.page_size - 1);
   p.pages64 = a.index_flags & KFMI_I64_PAGES;
   p.len64 = a.index_flags & KFMI_I64_LENGTHS;
-  p.scale = (float)a.scale;
-  p.softcap = (float)a.softcap;
+  constexpr double log2e = 1.4426950408889634;
+  p.score_scale = (float)(a.softcap > 0 ? 2.0 * log2e * a.scale / a.softcap : a.scale * log2e);
+  p.cap = (float)(a.softcap * log2e);
   const int64_t need = decode_workspace_bytes(a);
   if (need > 0 && a.work && a.work_bytes >= need) {
     p.counters = (int *)a.work;

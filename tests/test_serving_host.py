@@ -143,7 +143,7 @@ REFUSED = [
     (DECODE, _dec, dict(cap=-1.0), "softcap"), (DECODE, _dec, dict(cap=float("nan")), "softcap"),
     (DECODE, _dec, dict(window=-1), "window"), (DECODE, _dec, dict(wb=-1), "work_bytes"),
     (DECODE, _dec, dict(work=P + 4, wb=100), "work must be"), (DECODE, _dec, dict(vc=P + 2), "v_cache must be"),
-    (DECODE, _dec, dict(qs=(1, 8, 8)), "q strides"), (DECODE, _dec, dict(num=2 ** 62), "too many"),
+    (DECODE, _dec, dict(qs=(1, 8, 8)), "q strides"), (DECODE, _dec, dict(num=2 ** 31), "num_pages"),
     (READ, _read, dict(L=0), ">= 1"), (READ, _read, dict(L=2 ** 31), "2^31"), (READ, _read, dict(k=0), "k must not"),
     (READ, _read, dict(pages=P + 2), "pages must be 4"), (READ, _read, dict(B=65536), "65535"),
     (READ, _read, dict(max=2 ** 31), "2^30 keys"),
