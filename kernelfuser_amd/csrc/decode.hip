@@ -34,6 +34,7 @@ namespace {
 constexpr int WV = 4;            // waves per workgroup
 constexpr int NTHR = 64 * WV;
 constexpr int UNIT = 32 * WV;    // keys per unit of work
+constexpr uint32_t NO_SPLIT = 3;
 constexpr int SC1 = 16;          // cache policy of agent-coherent accesses
 
 struct DecodeParams {
@@ -47,7 +48,7 @@ struct DecodeParams {
   int64_t qs[3], cs[3], es[2];
   int64_t pages_stride, lengths_stride;
   int num_pages, B, hq, hk, S, group, rows, rblocks;  // rows = group * S, in blocks of 16 * NT
-  int capacity, window, min_units;
+  int capacity, window;
   int page_shift, page_mask;
   bool pages64, len64;
   float score_scale;  // of q . k: to the exponent of 2 (cap 0), or to the argument 2 y log2(e) of the capped one
@@ -124,6 +125,9 @@ __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t w, bool high) {
                                            : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, false));
 }
 
+// The high bits of the bytes that are 255.
+__device__ __forceinline__ uint32_t ff_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
+
 // The d that element (m, t) of O^T is: lane group m of V's loads, product t.
 template <int D, bool FP8>
 __device__ __forceinline__ int d_of(int m, int x) {  // of t = 8 * x
@@ -167,8 +171,10 @@ struct VTile {
   }
 };
 
-// Waves per SIMD that the registers of a step (K, V, Q, the accumulators) leave room for.
-constexpr int waves_per_simd(int d, bool fp8, int nt) { return d * nt * (fp8 ? 1 : d / 128) <= 256 ? 2 : 1; }
+// Waves per SIMD.  A wave alone on its SIMD reads bf16 as fast as two do, and half
+// the workgroups make half the parts of a split sequence; e4m3 takes twice the
+// arithmetic per byte and is faster with two waves where the registers allow them.
+constexpr int waves_per_simd(int d, bool fp8, int nt) { return fp8 && d * nt <= 256 ? 2 : 1; }
 
 // MULTI: S > 1.
 template <int D, bool FP8, int NT, bool MULTI>
@@ -176,6 +182,7 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
   constexpr int NK = D / 32;    // matrix steps of q . k
   constexpr int ND = D / 16;    // products of P V
   constexpr int NX = ND / 8;
+  constexpr int JU = D == 128 && !FP8 && NT <= 2 ? 2 : 1;  // parts in flight in the join
   constexpr int ES = FP8 ? 1 : 2;
   constexpr int ROWS = 16 * NT;
   constexpr int SLOT = ROWS * (D + 2);  // floats: O row by row, then (m, l) of each row
@@ -200,7 +207,13 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
     if (lane >= o) incl += y;
   }
   const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
-  const uint32_t per = max((total + gridDim.x - 1) / gridDim.x, (uint32_t)p.min_units);
+  // Sequences of up to NO_SPLIT units are left whole where there are fewer units
+  // than workgroups: a join takes as long as two or three units.
+  uint32_t most = p.B <= 64 && lane < p.B ? (uint32_t)sequence(p, lane).units : 0u;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
+  most = (uint32_t)__builtin_amdgcn_readfirstlane((int)most);
+  const uint32_t per = max((total + gridDim.x - 1) / gridDim.x, most <= NO_SPLIT ? most : 1u);
   const uint32_t g0 = blockIdx.x * per, g1 = min(g0 + per, total);
   if (g0 >= total) return;  // workgroup-uniform
   int b = __builtin_ctzll(__ballot(incl > g0));
@@ -357,12 +370,22 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
       }
       float ks[FP8 ? 8 : 1], vs[FP8 ? 8 : 1];
       if constexpr (FP8) {
+        const uint32_t odd = ff_bytes(ksw[0]) | ff_bytes(ksw[1]) | ff_bytes(vsw[0]) | ff_bytes(vsw[1]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          ks[i] = p.score_scale * scale_value((ksw[i / 4] >> (8 * (i & 3))) & 255u);
-          vs[i] = scale_value((vsw[i / 4] >> (8 * (i & 3))) & 255u);
-          const int j = j0 + 16 * (i / 4) + 4 * c + (i & 3);
-          if (edge && (j < s.lo || j >= s.len)) ks[i] = vs[i] = 0.f;  // one that is not seen may be NaN
+          const int sh = 8 * (i & 3);
+          ks[i] = __builtin_amdgcn_ldexpf(p.score_scale, (int)((ksw[i / 4] >> sh) & 255u) - 127);
+          vs[i] = __builtin_amdgcn_ldexpf(1.0f, (int)((vsw[i / 4] >> sh) & 255u) - 127);
+        }
+        if (edge || __any(odd != 0)) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int sh = 8 * (i & 3);
+            if (((ksw[i / 4] >> sh) & 255u) == 255u) ks[i] = __uint_as_float(0x7fc00000u);
+            if (((vsw[i / 4] >> sh) & 255u) == 255u) vs[i] = __uint_as_float(0x7fc00000u);
+            const int j = j0 + 16 * (i / 4) + 4 * c + (i & 3);
+            if (j < s.lo || j >= s.len) ks[i] = vs[i] = 0.f;  // one that is not seen may be NaN
+          }
         }
       }
       __builtin_amdgcn_sched_barrier(0);  // the loads take the registers of what they follow
@@ -581,28 +604,35 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
             sum[r] = 0.f;
           }
 #pragma unroll 1
-          for (uint32_t k = pgi; k < parts; k += pgs) {
-            const uint32_t from = w0 + k;
-            const uint32_t at = (2 * from + (from == w0 ? 1 : 0)) * (SLOT * 4);
-            u32x4_t po[4][2];
-            u32x2_t pm[4];
+          for (uint32_t k = pgi; k < parts; k += JU * pgs) {
+            u32x4_t po[JU][4][2];
+            u32x2_t pm[JU][4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int rr = min(r0 + r, rows_here - 1);
-              pm[r] = __builtin_amdgcn_raw_buffer_load_b64(all, at + (ROWS * D + 2 * rr) * 4, 0, SC1);
-              po[r][0] = __builtin_amdgcn_raw_buffer_load_b128(all, at + (rr * D + 8 * piece) * 4, 0, SC1);
-              po[r][1] = __builtin_amdgcn_raw_buffer_load_b128(all, at + (rr * D + 8 * piece + 4) * 4, 0, SC1);
+            for (int q = 0; q < JU; ++q) {
+              const uint32_t from = w0 + min(k + q * pgs, parts - 1);
+              const uint32_t at = (2 * from + (from == w0 ? 1 : 0)) * (SLOT * 4);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const int rr = min(r0 + r, rows_here - 1);
+                pm[q][r] = __builtin_amdgcn_raw_buffer_load_b64(all, at + (ROWS * D + 2 * rr) * 4, 0, SC1);
+                po[q][r][0] = __builtin_amdgcn_raw_buffer_load_b128(all, at + (rr * D + 8 * piece) * 4, 0, SC1);
+                po[q][r][1] = __builtin_amdgcn_raw_buffer_load_b128(all, at + (rr * D + 8 * piece + 4) * 4, 0, SC1);
+              }
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float pmax = __uint_as_float(pm[r][0]);
-              const float top = fmaxf(mm[r], pmax), base = top == -INFINITY ? 0.f : top;
-              const float a = __builtin_amdgcn_exp2f(mm[r] - base), a1 = __builtin_amdgcn_exp2f(pmax - base);
-              mm[r] = top;
-              sum[r] = fmaf(__uint_as_float(pm[r][1]), a1, sum[r] * a);
+            for (int q = 0; q < JU; ++q) {
+              if (k + q * pgs >= parts) break;
 #pragma unroll
-              for (int e = 0; e < 8; ++e) o[r][e] = fmaf(__uint_as_float(po[r][e / 4][e % 4]), a1, o[r][e] * a);
+              for (int r = 0; r < 4; ++r) {
+                const float pmax = __uint_as_float(pm[q][r][0]);
+                const float top = fmaxf(mm[r], pmax), base = top == -INFINITY ? 0.f : top;
+                const float a = __builtin_amdgcn_exp2f(mm[r] - base), a1 = __builtin_amdgcn_exp2f(pmax - base);
+                mm[r] = top;
+                sum[r] = fmaf(__uint_as_float(pm[q][r][1]), a1, sum[r] * a);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[r][e] = fmaf(__uint_as_float(po[q][r][e / 4][e % 4]), a1, o[r][e] * a);
+              }
             }
           }
           __syncthreads();
@@ -656,7 +686,7 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
 // Rows of a pass and workgroups of a launch.
 struct Plan {
   int nt, rblocks;
-  int64_t grid, slot_floats;
+  int64_t grid, slots, slot_floats;
 };
 
 Plan plan_of(const kfmi_decode_args &a) {
@@ -666,8 +696,9 @@ Plan plan_of(const kfmi_decode_args &a) {
   r.nt = rows <= 16 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
   r.rblocks = (int)((rows + 16 * r.nt - 1) / (16 * r.nt));
   const int64_t units = a.B * a.Hkv * r.rblocks * ((a.max_pages * a.page_size + UNIT - 1) / UNIT);
-  const int64_t round = 256 * waves_per_simd((int)a.D, a.cache_type == KFMI_CACHE_E4M3, r.nt);  // workgroups that run at once: two or one per CU
+  const int64_t round = 256 * waves_per_simd((int)a.D, a.cache_type == KFMI_CACHE_E4M3, r.nt);
   r.grid = units < round ? units : round;
+  r.slots = units < 512 ? units : 512;  // for either type of cache
   r.slot_floats = 16 * r.nt * (a.D + 2);
   return r;
 }
@@ -702,7 +733,7 @@ hipError_t dispatch_decode(const DecodeParams &p, int nt, int64_t grid, hipStrea
 
 int64_t decode_workspace_bytes(const kfmi_decode_args &a) {
   const Plan r = plan_of(a);
-  return r.grid > 1 ? KFMI_DECODE_COUNTER_BYTES + 2 * r.grid * r.slot_floats * 4 : 0;
+  return r.slots > 1 ? KFMI_DECODE_COUNTER_BYTES + 2 * r.slots * r.slot_floats * 4 : 0;
 }
 
 hipError_t launch_decode(const kfmi_decode_args &a, hipStream_t stream) {
@@ -722,7 +753,6 @@ hipError_t launch_decode(const kfmi_decode_args &a, hipStream_t stream) {
   p.num_pages = (int)a.num_pages;
   p.capacity = (int)(a.max_pages * a.page_size);
   p.window = (int)(a.window < p.capacity ? a.window : 0);  // a window of all keys is none
-  p.min_units = 1;
   p.B = (int)a.B; p.hq = (int)a.Hq; p.hk = (int)a.Hkv; p.S = (int)a.S;
   p.group = p.hq / p.hk;
   p.rows = p.group * p.S;
