@@ -34,7 +34,6 @@ namespace {
 constexpr int WV = 4;            // waves per workgroup
 constexpr int NTHR = 64 * WV;
 constexpr int UNIT = 32 * WV;    // keys per unit of work
-constexpr uint32_t NO_SPLIT = 3;
 constexpr int SC1 = 16;          // cache policy of agent-coherent accesses
 
 struct DecodeParams {
@@ -73,6 +72,22 @@ __device__ __forceinline__ Sequence sequence(const DecodeParams &p, int b) {
   s.start = s.lo & ~31;
   s.units = p.counters ? max(1, (s.len - s.start + UNIT - 1) / UNIT) : 1;  // never split: one unit of all keys
   return s;
+}
+
+// Units of work per workgroup: an even share, but
+//  * where two workgroups per CU would have up to four units each, one has
+//    them all (e4m3, 32 sequences of 1024 keys: 19.2 instead of 21.2 us at D = 128, 29.0
+//    instead of 32.0 at D = 256; from eight units on two are faster, 31.7 instead of 32.7);
+//  * a sequence (`most` units, the longest) of up to three units is not split: the join
+//    takes as long as two (one of 333 keys: 9.2 instead of 9.7 us), and a longer
+//    one not into more parts than its join, some 2.5 us for 64 rows of
+//    parts, leaves worth it: units / parts * 1.2 us + rows * parts / 64 * 2.5 us is least at
+//    parts = sqrt(31 * units / rows) (8192 keys, 32 rows: 66 us in 32 parts).
+__device__ __forceinline__ uint32_t units_per_workgroup(uint32_t total, uint32_t most, uint32_t grid, uint32_t rows) {
+  uint32_t even = (total + grid - 1) / grid;
+  if (grid > 256 && even <= 4) even = (total + 255) / 256;
+  const uint32_t least = most <= 3 ? most : min(most, (uint32_t)__builtin_sqrtf((float)(most * rows) * (1.0f / 31.0f)));
+  return max(even, max(least, 1u));
 }
 
 // A workgroup's part of one sequence, head and block of rows: units k0 .. k1 - 1.
@@ -198,22 +213,28 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
 
   // This workgroup's share [g0, g1) of all units, the sequences in the order
   // 0, 64, 128, .., 1, 65, .. (lane by lane); every wave finds it by itself.
-  uint32_t mine = 0;
-  for (int b = lane; b < p.B; b += 64) mine += (uint32_t)sequence(p, b).units * ipb;
-  uint32_t incl = mine;
+  uint32_t mine = 0, incl, most = 0;  // units of this lane's sequences, of all up to it; the longest's
+  if (p.B == 1) {
+    most = (uint32_t)sequence(p, 0).units;
+    mine = lane == 0 ? most * ipb : 0u;
+    incl = most * ipb;
+  } else {
+    for (int b = lane; b < p.B; b += 64) {
+      const uint32_t u = (uint32_t)sequence(p, b).units;
+      mine += u * ipb;
+      most = max(most, u);
+    }
+    incl = mine;
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const uint32_t y = (uint32_t)__shfl_up((int)incl, o);
-    if (lane >= o) incl += y;
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t y = (uint32_t)__shfl_up((int)incl, o);
+      if (lane >= o) incl += y;
+      most = max(most, (uint32_t)__shfl_xor((int)most, o));
+    }
   }
-  const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
-  // Sequences of up to NO_SPLIT units are left whole where there are fewer units
-  // than workgroups: a join takes as long as two or three units.
-  uint32_t most = p.B <= 64 && lane < p.B ? (uint32_t)sequence(p, lane).units : 0u;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, o));
   most = (uint32_t)__builtin_amdgcn_readfirstlane((int)most);
-  const uint32_t per = max((total + gridDim.x - 1) / gridDim.x, most <= NO_SPLIT ? most : 1u);
+  const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
+  const uint32_t per = units_per_workgroup(total, most, gridDim.x, (uint32_t)min(ROWS, p.rows));
   const uint32_t g0 = blockIdx.x * per, g1 = min(g0 + per, total);
   if (g0 >= total) return;  // workgroup-uniform
   int b = __builtin_ctzll(__ballot(incl > g0));
