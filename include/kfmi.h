@@ -428,7 +428,7 @@ typedef struct {
   int32_t top, logits_type, index_flags, reserved;
 } kfmi_logprobs_args;
 
-/* For each row x of logits (V < 2^31), in one pass over it:
+/* For each row x of logits (V < 2^30), in one pass over it:
  *   logprobs = x[id] - log sum exp x        (NaN for an id outside 0 .. V-1)
  *   entropy  = -sum p log p, p = softmax x  (p = 0 adds nothing)
  *   top_ids  = the `top` (0 .. 32, at most V) largest logits' indices, largest first,

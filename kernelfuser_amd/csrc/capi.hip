@@ -608,8 +608,8 @@ static int check_logprobs_shape(const kfmi_logprobs_args *a) {
   if (a->N0 < 1 || a->N1 < 1 || a->V < 1)
     return fail(KFMI_EINVAL, "N0, N1 and V must be >= 1 (got %lld, %lld, %lld)", (long long)a->N0, (long long)a->N1, (long long)a->V);
   const int64_t lim = (int64_t)1 << 31;
-  if (a->V >= lim || a->N0 >= lim || a->N1 >= lim || a->N0 * a->N1 >= lim / 64)
-    return fail(KFMI_EINVAL, "V must be below 2^31 and N0 * N1 below 2^25");
+  if (a->V >= lim / 2 || a->N0 >= lim || a->N1 >= lim || a->N0 * a->N1 >= lim / 64)
+    return fail(KFMI_EINVAL, "V must be below 2^30 and N0 * N1 below 2^25");
   if (a->logits_type < KFMI_LOGITS_F32 || a->logits_type > KFMI_LOGITS_F16)
     return fail(KFMI_EINVAL, "logits_type must be KFMI_LOGITS_F32, _BF16 or _F16 (got %d)", a->logits_type);
   if (a->top < 0 || a->top > KFMI_LOGPROBS_TOP_MAX || a->top > a->V)

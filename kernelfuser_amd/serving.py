@@ -420,8 +420,8 @@ def token_logprobs(logits, ids, top=0, *, work=None) -> TokenLogprobs:
         raise ValueError("Expected logits [...,V] with up to two leading dimensions and ids [...]")
     flags = _wide(ids, _lib.I64_IDS, "ids")
     v, top = logits.shape[-1], int(top)
-    if v < 1 or v >= 2 ** 31 or (v > 1 and logits.stride(-1) != 1):
-        raise ValueError("logits need contiguous rows of 1 to 2**31 - 1 values")
+    if v < 1 or v >= 2 ** 30 or (v > 1 and logits.stride(-1) != 1):
+        raise ValueError("logits need contiguous rows of 1 to 2**30 - 1 values")
     if not 0 <= top <= min(_lib.LOGPROBS_TOP_MAX, v):
         raise ValueError(f"top must be from 0 to {_lib.LOGPROBS_TOP_MAX} and at most V")
     n0, n1 = (1, 1, *lead)[-2:]

@@ -147,7 +147,7 @@ REFUSED = [
     (READ, _read, dict(L=0), ">= 1"), (READ, _read, dict(L=2 ** 31), "2^31"), (READ, _read, dict(k=0), "k must not"),
     (READ, _read, dict(pages=P + 2), "pages must be 4"), (READ, _read, dict(B=65536), "65535"),
     (READ, _read, dict(max=2 ** 31), "2^30 keys"),
-    (LOGPROBS, _lp, dict(v=0), ">= 1"), (LOGPROBS, _lp, dict(v=2 ** 31), "2^31"), (LOGPROBS, _lp, dict(n1=2 ** 26), "2^25"),
+    (LOGPROBS, _lp, dict(v=0), ">= 1"), (LOGPROBS, _lp, dict(v=2 ** 30), "2^30"), (LOGPROBS, _lp, dict(n1=2 ** 26), "2^25"),
     (LOGPROBS, _lp, dict(top=33), "top must"), (LOGPROBS, _lp, dict(top=-1), "top must"),
     (LOGPROBS, _lp, dict(v=2), "top must"), (LOGPROBS, _lp, dict(kind=3), "logits_type"),
     (LOGPROBS, _lp, dict(flags=1), "index_flags"), (LOGPROBS, _lp, dict(logits=P + 2), "logits must be 4"),
