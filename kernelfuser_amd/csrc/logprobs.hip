@@ -4,7 +4,8 @@
 // One pass over a row x: each lane keeps a running maximum m with
 //   z = sum e^(x - m),  t = sum e^(x - m) (x - m)
 // (rescaled when m grows: t' = a (t + (m - m') z), z' = a z, a = e^(m - m')),
-// so that logp = x[id] - m - log z and the entropy is log z - t / z.  The
+// so that logp = x[id] - m - log z and the entropy is log z - t / z; all of
+// it in units of log 2, which is what v_exp_f32 takes.  The
 // alternatives are one sorted list per wave, entry i in lane i, of
 // (value, index) as one whole number; a tile of logits is looked through only
 // where its maximum exceeds the list's last entry, which a row of random logits
@@ -28,6 +29,7 @@ constexpr int LU = 4;          // 16-byte loads of a lane in flight
 constexpr int MAX_SPLIT = 64;  // workgroups that share a row
 constexpr int MAX_ROWS = KFMI_LOGPROBS_COUNTER_BYTES / 4;  // rows of a launch that splits them
 constexpr int TOPM = KFMI_LOGPROBS_TOP_MAX;
+constexpr int WAVE_ROWS = 4096;  // rows from which each is one wave's: four waves per SIMD
 constexpr float L2E = 1.44269504088896340736f;
 
 // A workgroup's part of a split row.
@@ -44,7 +46,8 @@ struct LogprobsParams {
   Part *parts;
   int64_t ls[2], is[2];
   int64_t N1;
-  int V, top, splits, vecs_per_split;  // 16-byte vectors of a row per workgroup
+  int V, top, rows, splits, vecs_per_split;  // 16-byte vectors of a row per workgroup
+  int waves;                                 // of a row: 4, or 1 (never split)
   bool ids64;
 };
 
@@ -83,41 +86,106 @@ __device__ __forceinline__ void unpack(const u32x4_t &w, float *f) {
 
 // (value, index) in the order of the alternatives as one whole number: larger
 // values first, then lower indices; 0 stands for none (-infinity, NaN).  -0 counts as 0.
+__device__ __forceinline__ uint32_t value_key(float x) {
+  const uint32_t u = __float_as_uint(x + 0.0f);
+  return x > -INFINITY ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 0u;
+}
 __device__ __forceinline__ uint64_t rank_key(float x, uint32_t i) {
-  uint32_t u = __float_as_uint(x + 0.0f);
-  u = u & 0x80000000u ? ~u : u | 0x80000000u;
-  return x > -INFINITY ? ((uint64_t)u << 32) | (uint32_t)~i : 0ull;
+  const uint32_t u = value_key(x);
+  return u ? (uint64_t)u << 32 | (uint32_t)~i : 0ull;
 }
-__device__ __forceinline__ float key_value(uint64_t key) {
-  const uint32_t u = (uint32_t)(key >> 32);
-  return key == 0 ? -INFINITY : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+__device__ __forceinline__ float key_value(uint32_t u) {
+  return u == 0 ? -INFINITY : __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
+__device__ __forceinline__ float key_value(uint64_t key) { return key_value((uint32_t)(key >> 32)); }
 __device__ __forceinline__ uint64_t lane_of(uint64_t x, int lane) {
   return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32 |
          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane);
 }
 
+// The value of lane ^ M.
+template <int M>
+__device__ __forceinline__ uint32_t exchange32(uint32_t x, int lane) {
+  if constexpr (M == 1) return dpp_u32<DPP_QUAD_XOR1>(x);
+  else if constexpr (M == 2) return dpp_u32<DPP_QUAD_XOR2>(x);
+  else if constexpr (M == 4) return dpp_u32<0x1B>(dpp_u32<DPP_ROW_HALF_MIRROR>(x));  // 7 - i, then 3 - i in each quad
+  else if constexpr (M == 8) return dpp_u32<DPP_ROW_ROR8>(x);
+  else if constexpr (M == 15) return dpp_u32<DPP_ROW_MIRROR>(x);
+  else if constexpr (M == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return lane & 16 ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return lane & 32 ? r[0] : r[1];
+  }
+}
+template <int M>
+__device__ __forceinline__ uint64_t exchange(uint64_t x, int lane) {
+  return (uint64_t)exchange32<M>((uint32_t)(x >> 32), lane) << 32 | exchange32<M>((uint32_t)x, lane);
+}
+
+// One step of a bitonic network: lanes with `keep` take the larger of the two.
+template <int M>
+__device__ __forceinline__ uint64_t step(uint64_t x, int lane, bool keep) {
+  const uint64_t y = exchange<M>(x, lane);
+  return (x > y) == keep ? x : y;
+}
+template <int M>
+__device__ __forceinline__ uint64_t steps(uint64_t x, int lane, bool up) {  // a bitonic run of 2 M lanes, sorted
+  x = step<M>(x, lane, ((lane & M) == 0) != up);
+  if constexpr (M > 1) x = steps<M / 2>(x, lane, up);
+  return x;
+}
+// The 64 lanes' keys, smallest first.
+__device__ __forceinline__ uint64_t sort_up(uint64_t x, int lane) {
+  x = steps<1>(x, lane, (lane & 2) == 0);
+  x = steps<2>(x, lane, (lane & 4) == 0);
+  x = steps<4>(x, lane, (lane & 8) == 0);
+  x = steps<8>(x, lane, (lane & 16) == 0);
+  x = steps<16>(x, lane, (lane & 32) == 0);
+  return steps<32>(x, lane, true);
+}
+
+// The top-th largest of the lanes' values (ordered as whole numbers).
+template <int M>
+__device__ __forceinline__ uint32_t steps32(uint32_t x, int lane, bool up) {
+  const uint32_t y = exchange32<M>(x, lane);
+  x = ((lane & M) == 0) != up ? max(x, y) : min(x, y);
+  if constexpr (M > 1) x = steps32<M / 2>(x, lane, up);
+  return x;
+}
+__device__ __forceinline__ uint32_t nth_largest(uint32_t x, int lane, int top) {
+  x = steps32<1>(x, lane, (lane & 2) == 0);
+  x = steps32<2>(x, lane, (lane & 4) == 0);
+  x = steps32<4>(x, lane, (lane & 8) == 0);
+  x = steps32<8>(x, lane, (lane & 16) == 0);
+  x = steps32<16>(x, lane, (lane & 32) == 0);
+  x = steps32<32>(x, lane, false);
+  return (uint32_t)__builtin_amdgcn_readlane((int)x, top - 1);
+}
+
 // A sorted list over the lanes of a wave, largest first; tau is entry top - 1.
+// Keys are unique, so the order in which they arrive does not matter.
 struct TopList {
   uint64_t key, tau;
 
-  // The lanes' keys in order.
-  __device__ __forceinline__ void sort(uint64_t x, int lane, int top) {
-    int r = 0;
-#pragma unroll 8
-    for (int i = 0; i < 64; ++i) {
-      const uint64_t y = lane_of(x, i);
-      r += y > x || (y == x && i < lane) ? 1 : 0;
-    }
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_ds_permute(4 * r, (int)(uint32_t)x);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_ds_permute(4 * r, (int)(x >> 32));
-    key = (uint64_t)hi << 32 | lo;
+  // 64 more keys, smallest first.
+  __device__ __forceinline__ void merge_up(uint64_t x, int lane, int top) {
+    key = steps<32>(x > key ? x : key, lane, false);
     tau = lane_of(key, top - 1);
   }
-
-  // One candidate per lane (0: none); keys are unique.
+  // Another list.
+  __device__ __forceinline__ void merge(uint64_t x, int lane, int top) {
+    merge_up(exchange<32>(exchange<16>(exchange<15>(x, lane), lane), lane), lane, top);
+  }
+  // One key per lane (0: none): a few are put in one by one, some 250 cycles each,
+  // more by a sort, as long as five of them.
   __device__ __forceinline__ void insert(uint64_t x, int lane, int top) {
     uint64_t todo = __ballot(x > tau);
+    if (__builtin_popcountll(todo) > 5) {
+      merge_up(sort_up(x, lane), lane, top);
+      return;
+    }
     while (todo) {
       const int l = __builtin_ctzll(todo);
       const uint64_t c = lane_of(x, l);
@@ -131,26 +199,52 @@ struct TopList {
   }
 };
 
-// Running maximum and sums of one lane, wave or workgroup.
+// max of three; a NaN among them is ignored (as by fmaxf, for which the compiler first
+// makes each operand a quiet one: an instruction each).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+
+// Over the lanes of a wave.
+__device__ __forceinline__ float wave_max(float x, int lane) {
+  auto with = [&](uint32_t y) { x = fmaxf(x, __uint_as_float(y)); };
+  with(exchange32<1>(__float_as_uint(x), lane));
+  with(exchange32<2>(__float_as_uint(x), lane));
+  with(exchange32<4>(__float_as_uint(x), lane));
+  with(exchange32<8>(__float_as_uint(x), lane));
+  with(exchange32<16>(__float_as_uint(x), lane));
+  with(exchange32<32>(__float_as_uint(x), lane));
+  return x;
+}
+__device__ __forceinline__ float wave_sum(float x, int lane) {
+  auto with = [&](uint32_t y) { x += __uint_as_float(y); };
+  with(exchange32<1>(__float_as_uint(x), lane));
+  with(exchange32<2>(__float_as_uint(x), lane));
+  with(exchange32<4>(__float_as_uint(x), lane));
+  with(exchange32<8>(__float_as_uint(x), lane));
+  with(exchange32<16>(__float_as_uint(x), lane));
+  with(exchange32<32>(__float_as_uint(x), lane));
+  return x;
+}
+
+// Running maximum and sums of one lane, wave or workgroup, in units of log 2:
+// y = x log2(e), z = sum 2^(y - m), t = sum 2^(y - m) (y - m).
 struct Sums {
   float m, z, t;
   __device__ __forceinline__ void move(float to) {  // to >= m; to -infinity only from -infinity
-    const float base = to == -INFINITY ? 0.f : to;
-    const float dm = m == -INFINITY ? 0.f : fmaxf(m - base, -1e4f);  // finite, for the product with a = 0
-    const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(dm * L2E);
+    // finite, for the product with a = 0; NaN (m and `to` are +infinity) meets a z that is NaN
+    const float dm = m == -INFINITY ? 0.f : fmaxf(m - to, -1e4f);
+    const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(dm);
     t = a * fmaf(dm, z, t);
     z = a * z;
     m = to;
   }
-  __device__ __forceinline__ void join(Sums o) {
-    const float to = fmaxf(m, o.m);
-    // a NaN in z or t (a row that is no distribution) goes through the sums
-    Sums a = *this;
-    a.move(to);
-    o.move(to);
-    m = to;
-    z = a.z + o.z;
-    t = a.t + o.t;
+  __device__ __forceinline__ void over_lanes(int lane) {
+    move(wave_max(m, lane));
+    z = wave_sum(z, lane);
+    t = wave_sum(t, lane);
   }
 };
 
@@ -159,12 +253,16 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
   constexpr int VEC = vec_of<TYPE>();
   constexpr int SIZE = 16 / VEC;
   constexpr int NE = LU * VEC;  // logits of a lane and tile
-  __shared__ uint64_t keys[4 * TOPM];
+  __shared__ uint64_t keys[4][TOPM];
+  __shared__ uint64_t found[TOP ? 4 : 1][TOP ? 64 + 64 * VEC : 1];
   __shared__ float sums[4][3];
   __shared__ uint32_t arrived;
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int row = (int)(blockIdx.x / (uint32_t)p.splits), part = (int)(blockIdx.x % (uint32_t)p.splits);
+  const bool alone = p.waves == 1;  // a row is one wave's, and no wave meets another
+  const int row = alone ? (int)blockIdx.x * 4 + w : (int)(blockIdx.x / (uint32_t)p.splits);
+  const int part = alone ? 0 : (int)(blockIdx.x % (uint32_t)p.splits);
+  if (alone && row >= p.rows) return;
   const int64_t n0 = row / p.N1, n1 = row - n0 * p.N1;
   const int64_t base = n0 * p.ls[0] + n1 * p.ls[1];
   const char *first = reinterpret_cast<const char *>(p.logits) + base * SIZE;
@@ -176,8 +274,8 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
 
   Sums s{-INFINITY, 0.f, 0.f};
   TopList list{0ull, 0ull};
-  bool begun = false;
-  for (int vt = v0 + w * (64 * LU); vt < v1; vt += 4 * 64 * LU) {
+  bool ruled_out = false;  // wave-uniform
+  for (int vt = v0 + (alone ? 0 : w) * (64 * LU); vt < v1; vt += p.waves * 64 * LU) {
     float x[NE];
     u32x4_t raw[LU];
     const bool inner = vt * VEC >= head && (vt + 64 * LU) * VEC - head <= p.V && vt + 64 * LU <= v1;  // wave-uniform
@@ -206,82 +304,104 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
     float vm[LU], top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < LU; ++u) {
-      vm[u] = x[u * VEC];
+      vm[u] = max3(x[u * VEC], x[u * VEC + 1], x[u * VEC + 2]);
+      if constexpr (VEC == 8) vm[u] = max3(max3(vm[u], x[u * VEC + 3], x[u * VEC + 4]), x[u * VEC + 5], x[u * VEC + 6]);
+    }
 #pragma unroll
-      for (int e = 1; e < VEC; ++e) vm[u] = fmaxf(vm[u], x[u * VEC + e]);
+    for (int u = 0; u < LU; ++u) {
+      vm[u] = fmaxf(vm[u], x[u * VEC + VEC - 1]);
       top = fmaxf(top, vm[u]);
     }
-    if (top > s.m) s.move(top);
+    if (top * L2E > s.m) s.move(top * L2E);
     const float b = s.m == -INFINITY ? 0.f : s.m;
+    // 0 * -infinity is NaN: a wave that meets -infinity does the tile again and goes on with the exponents
+    // held above -1000, which costs an instruction per logit.
+    const Sums kept = s;
+    if (!ruled_out) {
+#pragma unroll
+      for (int i = 0; i < NE; ++i) {
+        const float d = fmaf(x[i], L2E, -b), e = __builtin_amdgcn_exp2f(d);
+        s.z += e;
+        s.t = fmaf(e, d, s.t);
+      }
+      ruled_out = __any(s.t != s.t);
+      if (ruled_out) s = kept;
+      else goto summed;
+    }
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
-      const float d = x[i] - b, e = __builtin_amdgcn_exp2f(d * L2E);
+      const float d = fmaf(x[i], L2E, -b), e = __builtin_amdgcn_exp2f(d);
       s.z += e;
-      s.t = fmaf(e, fmaxf(d, -1000.0f), s.t);  // e is 0 (or NaN) where this matters
+      s.t = fmaf(e, fmaxf(d, -1000.0f), s.t);
     }
+  summed:
     if constexpr (TOP) {
       const uint32_t i0 = (uint32_t)((vt + lane) * VEC - head);  // index of x[0]
-      if (!begun) {
-        begun = true;
-        // the lane's largest, the first of equals
-        float best = x[0];
-        int at = 0;
+      if (__any(top > key_value(list.tau))) {
+        // What may belong is gathered in LDS and enters the list 64 at a time.  In
+        // the first tile that is what reaches the top-th largest of the lanes' maxima,
+        // later what exceeds the list's last entry (an equal one has a higher index).
+        const bool begin = list.tau == 0;
+        const float tv = key_value(begin ? nth_largest(value_key(top), lane, p.top) : (uint32_t)(list.tau >> 32));
+        auto belongs = [&](float y) { return (y > tv || (begin && y == tv)) && y > -INFINITY; };
+        int have = 0;
+        auto flush = [&] {
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          for (int o = 0; o < have; o += 64) list.insert(o + lane < have ? found[w][o + lane] : 0ull, lane, p.top);
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          have = 0;
+        };
 #pragma unroll
-        for (int i = 1; i < NE; ++i) {
-          const bool more = x[i] > best || !(best > -INFINITY);
-          best = more ? x[i] : best;
-          at = more ? i : at;
-        }
-        const uint32_t bi = i0 + (uint32_t)(at / VEC * 64 * VEC + at % VEC);
-        list.sort(rank_key(best, bi), lane, p.top);
-        const float tv = key_value(list.tau);
-        if (__any(top >= tv && top > -INFINITY)) {
+        for (int u = 0; u < LU; ++u) {
+          if (!__any(belongs(vm[u]))) continue;
+          if (have > 64) flush();
 #pragma unroll
-          for (int u = 0; u < LU; ++u) {
-            if (!__any(vm[u] >= tv && vm[u] > -INFINITY)) continue;
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-              const uint32_t i = i0 + (uint32_t)(u * 64 * VEC + e);
-              const uint64_t key = i == bi ? 0ull : rank_key(x[u * VEC + e], i);
-              list.insert(key, lane, p.top);
+          for (int e = 0; e < VEC; ++e) {
+            const float y = x[u * VEC + e];
+            const bool in = belongs(y);
+            const uint64_t ins = __ballot(in);
+            if (ins) {
+              if (in) found[w][have + __builtin_popcountll(ins & ((1ull << lane) - 1))] = rank_key(y, i0 + (uint32_t)(u * 64 * VEC + e));
+              have += __builtin_popcountll(ins);
             }
           }
         }
-      } else if (__any(top > key_value(list.tau))) {
-#pragma unroll
-        for (int u = 0; u < LU; ++u) {
-          if (!__any(vm[u] > key_value(list.tau))) continue;
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const uint32_t i = i0 + (uint32_t)(u * 64 * VEC + e);
-            if (__any(x[u * VEC + e] > key_value(list.tau))) list.insert(rank_key(x[u * VEC + e], i), lane, p.top);
-          }
-        }
+        flush();
       }
     }
   }
 
-  auto join_waves = [&](Sums x) {  // x of the wave's lanes, then of the waves
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) x.join(Sums{__shfl_xor(x.m, o), __shfl_xor(x.z, o), __shfl_xor(x.t, o)});
+  // The lanes' sums and lists of all waves, in the first wave (lists: each wave's in LDS).
+  auto join_waves = [&](Sums x) {
+    x.over_lanes(lane);
+    if (alone) return x;
     if (lane == 0) {
       sums[w][0] = x.m;
       sums[w][1] = x.z;
       sums[w][2] = x.t;
     }
-    if (TOP && lane < p.top) keys[w * p.top + lane] = list.key;
+    if (TOP && lane < p.top) keys[w][lane] = list.key;
     __syncthreads();
-    x = Sums{sums[0][0], sums[0][1], sums[0][2]};
+    if (w == 0) {
+      const float top = fmaxf(fmaxf(sums[0][0], sums[1][0]), fmaxf(sums[2][0], sums[3][0]));
+      float z = 0.f, t = 0.f;
 #pragma unroll
-    for (int i = 1; i < 4; ++i) x.join(Sums{sums[i][0], sums[i][1], sums[i][2]});
+      for (int i = 0; i < 4; ++i) {
+        Sums y{sums[i][0], sums[i][1], sums[i][2]};
+        y.move(top);
+        z += y.z;
+        t += y.t;
+      }
+      x = Sums{top, z, t};
+    }
     return x;
   };
-  // This thread's key of the four lists and its place among them all.
-  auto place = [&](uint64_t &key) {
-    key = tid < 4 * p.top ? keys[tid] : 0ull;
-    int r = 0;
-    for (int i = 0; i < 4 * p.top; ++i) r += keys[i] > key ? 1 : 0;
-    return r;
+  // The waves' lists as one, in the first wave.
+  auto join_lists = [&] {
+    if (TOP && w == 0 && !alone) {
+#pragma unroll
+      for (int i = 1; i < 4; ++i) list.merge(lane < p.top ? keys[i][lane] : 0ull, lane, p.top);
+    }
   };
 
   Sums all = join_waves(s);
@@ -289,14 +409,8 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
     // Parts are written and read with agent-coherent accesses and the last
     // workgroup of a row joins them, as in the decode kernel.
     Part *mine = p.parts + (int64_t)row * p.splits + part;
-    if constexpr (TOP) {
-      uint64_t key;
-      const int r = place(key);
-      if (key != 0 && r < p.top) __hip_atomic_store(&mine->keys[r], key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      // places that no key takes: there are fewer keys than `top`
-      const int have = __syncthreads_count(key != 0);
-      if (tid >= have && tid < p.top) __hip_atomic_store(&mine->keys[tid], 0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    join_lists();
+    if (TOP && tid < p.top) __hip_atomic_store(&mine->keys[tid], list.key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (tid == 0) {
       __hip_atomic_store(&mine->m, all.m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       __hip_atomic_store(&mine->z, all.z, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -317,58 +431,52 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
     }
     if constexpr (TOP) {
       list = TopList{0ull, 0ull};
-      const int n = p.splits * p.top;
-      for (int i = w * 64; i < n; i += 256) {
-        uint64_t key = 0;
-        if (i + lane < n)
-          key = __hip_atomic_load(&parts[(i + lane) / p.top].keys[(i + lane) % p.top], __ATOMIC_RELAXED,
-                                  __HIP_MEMORY_SCOPE_AGENT);
-        if (i == w * 64) list.sort(key, lane, p.top);
-        else list.insert(key, lane, p.top);
-      }
+      for (int i = w; i < p.splits; i += 4)
+        list.merge(lane < p.top ? __hip_atomic_load(&parts[i].keys[min(lane, TOPM - 1)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                                : 0ull, lane, p.top);
     }
     if (tid == 0) __hip_atomic_store(p.counters + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     all = join_waves(s);
   }
 
+  if (w != 0 && !alone) return;
+  constexpr float LN2 = 0.693147180559945309417f;
   const float nan = __uint_as_float(0x7fc00000u);
   const bool none = !(all.z > 0.f);  // NaN, +infinity or no logit above -infinity
-  const float lse = logf(all.z);
-  if (tid == 0) {
+  const float lz = log2f(all.z);
+  auto logp = [&](float x) { return (fmaf(x, L2E, -all.m) - lz) * LN2; };
+  if (lane == 0) {
     const int64_t id = load_index(p.ids, p.ids64, n0 * p.is[0] + n1 * p.is[1]);
     const bool in = id >= 0 && id < p.V;
-    p.logprobs[row] = none || !in ? nan : load_logit<TYPE>(first, in ? id : 0) - all.m - lse;
-    p.entropy[row] = none ? nan : lse - all.t / all.z;
+    p.logprobs[row] = none || !in ? nan : logp(load_logit<TYPE>(first, in ? id : 0));
+    p.entropy[row] = none ? nan : (lz - all.t / all.z) * LN2;
   }
   if constexpr (TOP) {
-    uint64_t key;
-    const int r = place(key);
+    join_lists();
     const int64_t out = (int64_t)row * p.top;
-    const int have = __syncthreads_count(key != 0);
     if (none) {
-      if (tid < p.top) {
-        p.top_ids[out + tid] = -1;
-        p.top_logprobs[out + tid] = nan;
+      if (lane < p.top) {
+        p.top_ids[out + lane] = -1;
+        p.top_logprobs[out + lane] = nan;
       }
-    } else {
-      if (key != 0 && r < p.top) {
-        p.top_ids[out + r] = (int64_t)(uint32_t)~(uint32_t)key;
-        p.top_logprobs[out + r] = key_value(key) - all.m - lse;
+      return;
+    }
+    if (lane < p.top && list.key != 0) {
+      p.top_ids[out + lane] = (int64_t)(uint32_t)~(uint32_t)list.key;
+      p.top_logprobs[out + lane] = logp(key_value(list.key));
+    }
+    // the lowest indices of -infinity take the places left
+    int at = __builtin_popcountll(__ballot(list.key != 0));
+    for (int i0 = 0; at < p.top && i0 < p.V; i0 += 64) {
+      const int i = i0 + lane;
+      const bool hit = i < p.V && load_logit<TYPE>(first, i < p.V ? i : 0) == -INFINITY;
+      const uint64_t hits = __ballot(hit);
+      const int to = at + __builtin_popcountll(hits & ((1ull << lane) - 1));
+      if (hit && to < p.top) {
+        p.top_ids[out + to] = i;
+        p.top_logprobs[out + to] = -INFINITY;
       }
-      if (w == 0) {  // the lowest indices of -infinity take the places left
-        int at = have;
-        for (int i = lane; at < p.top; i += 64) {
-          const bool hit = i < p.V && load_logit<TYPE>(first, i < p.V ? i : 0) == -INFINITY;
-          const uint64_t hits = __ballot(hit);
-          const int to = at + __builtin_popcountll(hits & ((1ull << lane) - 1));
-          if (hit && to < p.top) {
-            p.top_ids[out + to] = i;
-            p.top_logprobs[out + to] = -INFINITY;
-          }
-          at += __builtin_popcountll(hits);
-          if (i - lane >= p.V) break;
-        }
-      }
+      at += __builtin_popcountll(hits);
     }
   }
 }
@@ -386,7 +494,7 @@ int splits_of(const kfmi_logprobs_args &a) {
 
 template <int TYPE, bool TOP>
 hipError_t launch_logprobs_t(const LogprobsParams &p, int64_t rows, hipStream_t stream) {
-  const int64_t grid = rows * p.splits;
+  const int64_t grid = p.waves == 1 ? (rows + 3) / 4 : rows * p.splits;
   hipLaunchKernelGGL((logprobs_kernel<TYPE, TOP>), dim3((unsigned)grid), dim3(256), 0, stream, p);
   static const std::string name = [] {
     char b[96];
@@ -394,7 +502,7 @@ hipError_t launch_logprobs_t(const LogprobsParams &p, int64_t rows, hipStream_t 
     return std::string(b);
   }();
   launch_log_add(reinterpret_cast<const void *>(&logprobs_kernel<TYPE, TOP>), name.c_str(), grid, 256);
-  launch_log_plan("splits=%d", p.splits);
+  launch_log_plan("splits=%d waves=%d", p.splits, p.waves);
   return hipGetLastError();
 }
 
@@ -422,7 +530,9 @@ hipError_t launch_logprobs(const kfmi_logprobs_args &a, hipStream_t stream) {
   p.V = (int)a.V;
   p.top = a.top;
   p.ids64 = a.index_flags & KFMI_I64_IDS;
+  p.rows = (int)(a.N0 * a.N1);
   p.splits = 1;
+  p.waves = p.rows >= WAVE_ROWS ? 1 : 4;
   const int64_t need = logprobs_workspace_bytes(a);
   if (need > 0 && a.work && a.work_bytes >= need) {
     p.splits = splits_of(a);
