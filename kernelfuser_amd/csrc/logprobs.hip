@@ -29,7 +29,7 @@ constexpr int LU = 4;          // 16-byte loads of a lane in flight
 constexpr int MAX_SPLIT = 64;  // workgroups that share a row
 constexpr int MAX_ROWS = KFMI_LOGPROBS_COUNTER_BYTES / 4;  // rows of a launch that splits them
 constexpr int TOPM = KFMI_LOGPROBS_TOP_MAX;
-constexpr int WAVE_ROWS = 4096;  // rows from which each is one wave's: four waves per SIMD
+constexpr int WAVE_ROWS = 1024;  // rows from which each is one wave's: a wave per SIMD
 constexpr float L2E = 1.44269504088896340736f;
 
 // A workgroup's part of a split row.
@@ -275,15 +275,22 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
   Sums s{-INFINITY, 0.f, 0.f};
   TopList list{0ull, 0ull};
   bool ruled_out = false;  // wave-uniform
-  for (int vt = v0 + (alone ? 0 : w) * (64 * LU); vt < v1; vt += p.waves * 64 * LU) {
-    float x[NE];
-    u32x4_t raw[LU];
-    const bool inner = vt * VEC >= head && (vt + 64 * LU) * VEC - head <= p.V && vt + 64 * LU <= v1;  // wave-uniform
-    if (inner) {
+  // Whether a tile lies within the row (wave-uniform), and its loads, which run while the
+  // tile before it is summed.
+  auto inner = [&](int vt) { return vt * VEC >= head && (vt + 64 * LU) * VEC - head <= p.V && vt + 64 * LU <= v1; };
+  u32x4_t raw[LU];
+  auto request = [&](int vt) {
 #pragma unroll
-      for (int u = 0; u < LU; ++u)
-        raw[u] = __builtin_nontemporal_load(
-            reinterpret_cast<const u32x4_t *>(first - head * SIZE + (int64_t)(vt + 64 * u + lane) * 16));
+    for (int u = 0; u < LU; ++u)
+      raw[u] = __builtin_nontemporal_load(
+          reinterpret_cast<const u32x4_t *>(first - head * SIZE + (int64_t)(vt + 64 * u + lane) * 16));
+  };
+  const int vt0 = v0 + (alone ? 0 : w) * (64 * LU), stride = p.waves * 64 * LU;
+  bool requested = vt0 < v1 && inner(vt0);
+  if (requested) request(vt0);
+  for (int vt = vt0; vt < v1; vt += stride) {
+    float x[NE];
+    if (requested) {
 #pragma unroll
       for (int u = 0; u < LU; ++u) unpack<TYPE>(raw[u], x + u * VEC);
     } else {
@@ -301,6 +308,8 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
         }
       }
     }
+    requested = vt + stride < v1 && inner(vt + stride);
+    if (requested) request(vt + stride);
     float vm[LU], top = -INFINITY;
 #pragma unroll
     for (int u = 0; u < LU; ++u) {
@@ -313,7 +322,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
       top = fmaxf(top, vm[u]);
     }
     if (top * L2E > s.m) s.move(top * L2E);
-    const float b = s.m == -INFINITY ? 0.f : s.m;
+    float b = s.m == -INFINITY ? 0.f : s.m;
     // 0 * -infinity is NaN: a wave that meets -infinity does the tile again and goes on with the exponents
     // held above -1000, which costs an instruction per logit.
     const Sums kept = s;
@@ -327,6 +336,8 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
       ruled_out = __any(s.t != s.t);
       if (ruled_out) s = kept;
       else goto summed;
+      // computed again, not kept: 64 registers
+      asm volatile("" : "+v"(b));
     }
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
@@ -431,9 +442,17 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
     }
     if constexpr (TOP) {
       list = TopList{0ull, 0ull};
-      for (int i = w; i < p.splits; i += 4)
-        list.merge(lane < p.top ? __hip_atomic_load(&parts[i].keys[min(lane, TOPM - 1)], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
-                                : 0ull, lane, p.top);
+      for (int i = w; i < p.splits; i += 16) {  // four lists on their way at once
+        uint64_t part_keys[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          part_keys[q] = lane < p.top && i + 4 * q < p.splits
+                             ? __hip_atomic_load(&parts[i + 4 * q].keys[lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)
+                             : 0ull;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (i + 4 * q < p.splits) list.merge(part_keys[q], lane, p.top);
+      }
     }
     if (tid == 0) __hip_atomic_store(p.counters + row, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     all = join_waves(s);
@@ -481,13 +500,14 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
   }
 }
 
-// Workgroups per row: enough for four per CU, each with a tile per wave at least.
+// Workgroups per row: two per CU, each with a tile per wave at least (64 rows of 131071 in 32 bits:
+// 10.8 us; with four per CU 12.8, with one 13.3).
 int splits_of(const kfmi_logprobs_args &a) {
   const int64_t rows = a.N0 * a.N1;
   if (rows > MAX_ROWS) return 1;
   const int64_t vec = a.logits_type == KFMI_LOGITS_F32 ? 4 : 8;
   const int64_t tiles = (a.V + vec * 64 * LU * 4 - 1) / (vec * 64 * LU * 4);
-  int64_t n = (1024 + rows - 1) / rows;
+  int64_t n = (512 + rows - 1) / rows;
   n = n < tiles ? n : tiles;
   return (int)(n < 1 ? 1 : n > MAX_SPLIT ? MAX_SPLIT : n);
 }
