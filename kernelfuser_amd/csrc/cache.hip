@@ -23,12 +23,14 @@ struct WriteParams {
   int64_t ps[2], ss[2];
   int64_t cs[3], es[2];
   uint32_t S, T, hq, hk;  // T = B * S tokens; heads of q (0: none) and of k
-  uint32_t rows;          // T * (hq + 2 * hk)
   int64_t table_rows, slot_end;
   int page_shift, page_mask;
   bool pos64, slot64;
   float eps;
 };
+
+// Rows from which a lane takes four heads of its token instead of one.
+constexpr int64_t WIDE_ROWS = 1 << 15;
 
 // A row of 8 values per lane in e4m3 with its scale 2^e: e is the smallest
 // exponent (at least -124: e4m3's smallest step, 2^-9, times 2^-124 is bf16's) with max|row| <= 448 * 2^e over the finite values, so that the
@@ -41,21 +43,32 @@ template <int LPR>
 __device__ __forceinline__ u32x2_t quantise_row(const float (&y)[8], uint32_t &byte) {
   uint32_t top = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t a = __float_as_uint(y[j]) & 0x7fffffffu;
-    top = max(top, a < 0x7f800000u ? a : 0u);
-  }
+  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(y[j]) & 0x7fffffffu);
   top = row_max_u32<LPR>(top);
+  const bool large = __any(top >= 0x7f000000u);  // 2^127 and more, infinities, NaN: rarely
+  if (large) {
+    top = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t a = __float_as_uint(y[j]) & 0x7fffffffu;
+      top = max(top, a < 0x7f800000u ? a : 0u);
+    }
+    top = row_max_u32<LPR>(top);
+  }
   const int ex = (int)(top >> 23) - 126 - 9 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
   const int e = top == 0 ? 0 : max(ex, -124);
   byte = (uint32_t)(e + 127);
   const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-  const float most = e == 120 ? 240.0f : 448.0f;
   float z[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    z[j] = __builtin_amdgcn_fmed3f(y[j] * inv, -most, most);
-    if ((__float_as_uint(y[j]) & 0x7f800000u) == 0x7f800000u) z[j] = __uint_as_float(0x7fc00000u);
+  for (int j = 0; j < 8; ++j) z[j] = y[j] * inv;
+  if (large) {
+    const float most = e == 120 ? 240.0f : 448.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      z[j] = __builtin_amdgcn_fmed3f(z[j], -most, most);
+      if ((__float_as_uint(y[j]) & 0x7f800000u) == 0x7f800000u) z[j] = __uint_as_float(0x7fc00000u);
+    }
   }
   u32x2_t w;
 #pragma unroll
@@ -67,101 +80,133 @@ __device__ __forceinline__ u32x2_t quantise_row(const float (&y)[8], uint32_t &b
   return w;
 }
 
-// One row per LPR lanes; rows in the order (head, token), heads of q, then k,
-// then v, so that neighbouring rows are neighbouring tokens of one head (or, for a few
-// tokens, neighbouring heads).
-template <int D, int ST, bool ROPE, bool FP8>
+// A workgroup takes 256 / LPR consecutive tokens (blockIdx.x) of a unit of U
+// heads of q, of k or of v (blockIdx.y), one 16-byte chunk per lane and row.  A lane's U
+// rows share the token's table rows, gamma, position and slot.  Every load is
+// issued before the first is waited for, and every row is finished before one is stored
+// (stores and loads share a counter).
+template <int D, int ST, bool ROPE, bool FP8, int U>
 __global__ __launch_bounds__(256) void cache_write_kernel(WriteParams p) {
   constexpr int LPR = D / 8;
   constexpr int HALF = LPR / 2;
-  const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  const uint32_t lc = threadIdx.x % LPR;
-  const bool live = row < p.rows;
-  const uint32_t r = live ? row : p.rows - 1;  // loads stay in bounds; nothing is stored for this lane
-  const uint32_t head = r / p.T, t = r - head * p.T;
+  const uint32_t t_ = blockIdx.x * (256 / LPR) + threadIdx.x / LPR, lc = threadIdx.x % LPR;
+  const bool live = t_ < p.T;
+  const uint32_t t = live ? t_ : p.T - 1;  // loads stay in bounds; nothing is stored for this lane
   const uint32_t b = t / p.S, s = t - b * p.S;
-  const bool is_q = head < p.hq, is_v = head >= p.hq + p.hk;
-  const uint32_t h = is_q ? head : is_v ? head - p.hq - p.hk : head - p.hq;
+  const uint32_t uq = (p.hq + U - 1) / U, uk = (p.hk + U - 1) / U;
+  const uint32_t unit = blockIdx.y;  // everything from here to the row is workgroup-uniform
+  const bool is_q = unit < uq, is_v = unit >= uq + uk;
+  const uint32_t nh = is_q ? p.hq : p.hk;
+  const uint32_t h0 = (is_q ? unit : is_v ? unit - uq - uk : unit - uq) * U;
   const uint16_t *src = is_q ? p.q : is_v ? p.v : p.k;
   const int64_t s0 = is_q ? p.qs[0] : is_v ? p.vs[0] : p.ks[0];
   const int64_t s1 = is_q ? p.qs[1] : is_v ? p.vs[1] : p.ks[1];
   const int64_t s2 = is_q ? p.qs[2] : is_v ? p.vs[2] : p.ks[2];
-  const u32x4_t xw = ld16_nt(src + b * s0 + h * s1 + s * s2 + lc * 8);
+  const uint16_t *row = src + b * s0 + s * s2 + lc * 8;
+  u32x4_t held[U];  // the row as it is, then prepared
+#pragma unroll
+  for (int i = 0; i < U; ++i) held[i] = ld16_nt(row + min(h0 + i, nh - 1) * s1);
   const int64_t slot = load_index(p.slots, p.slot64, b * p.ss[0] + s * p.ss[1]);
-  const u32x4_t gw = ld16((is_q ? p.gq : p.gk) + lc * 8);
-  bool bad_pos = false;
-  u32x4_t cw, sw;
-  if constexpr (ROPE) {
-    int64_t pos = load_index(p.positions, p.pos64, b * p.ps[0] + s * p.ps[1]);
-    bad_pos = pos < 0 || pos >= p.table_rows;
-    pos = bad_pos ? 0 : pos;
-    cw = ld16(p.cos + pos * D + lc * 8);
-    sw = ld16(p.sin + pos * D + lc * 8);
-  }
   const bool bad_slot = slot >= p.slot_end;
-  float x[8], y[8];
-  unpack8(xw, x);
-  float g[8];
-  unpack8(gw, g);
-  const float inv = row_inv_rms<LPR, D>(x, p.eps);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) y[j] = norm_elem<ST>(x[j], inv, g[j]);
-  if constexpr (ROPE) {
-    const uint32_t flip = lc < HALF ? 0x80008000u : 0u;  // first half: n*c - np*s
-    sw ^= u32x4_t{flip, flip, flip, flip};
-    float c[8], sn[8];
-    unpack8(cw, c);
-    unpack8(sw, sn);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = rope_elem<ST>(y[j], partner_f32<LPR>(y[j]), c[j], sn[j], false);
-  }
-  u32x4_t yw = pack8(y);
   const uint32_t nan2 = 0x7fc07fc0u;
-  if (bad_pos) yw = u32x4_t{nan2, nan2, nan2, nan2};
-  const u32x4_t held = is_v ? xw : yw;  // what the cache holds
-  u32x2_t payload;
-  uint32_t byte = 0;
+  if (!is_v) {
+    const u32x4_t gw = ld16((is_q ? p.gq : p.gk) + lc * 8);
+    bool bad_pos = false;
+    u32x4_t cw, sw;
+    if constexpr (ROPE) {
+      int64_t pos = load_index(p.positions, p.pos64, b * p.ps[0] + s * p.ps[1]);
+      bad_pos = pos < 0 || pos >= p.table_rows;
+      pos = bad_pos ? 0 : pos;
+      cw = ld16(p.cos + pos * D + lc * 8);
+      sw = ld16(p.sin + pos * D + lc * 8);
+    }
+    asm volatile("" ::: "memory");
+    float g[8], c[8], sn[8];
+    unpack8(gw, g);
+    if constexpr (ROPE) {
+      const uint32_t flip = lc < HALF ? 0x80008000u : 0u;  // first half: n*c - np*s
+      sw ^= u32x4_t{flip, flip, flip, flip};
+      unpack8(cw, c);
+      unpack8(sw, sn);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      float x[8], y[8];
+      unpack8(held[i], x);
+      const float inv = row_inv_rms<LPR, D>(x, p.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = norm_elem<ST>(x[j], inv, g[j]);
+      if constexpr (ROPE) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = rope_elem<ST>(y[j], partner_f32<LPR>(y[j]), c[j], sn[j], false);
+      }
+      held[i] = pack8(y);
+      if (bad_pos) held[i] = u32x4_t{nan2, nan2, nan2, nan2};
+      asm volatile("" ::"v"(held[i]));  // finished here, with every lane active, not in the stores' branches
+    }
+  }
+  u32x2_t payload[U];
+  uint32_t byte[U];
   if constexpr (FP8) {
-    float f[8];
-    unpack8(held, f);
-    payload = quantise_row<LPR>(f, byte);
+    if (!is_q) {
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        float f[8];
+        unpack8(held[i], f);
+        payload[i] = quantise_row<LPR>(f, byte[i]);
+        asm volatile("" ::"v"(payload[i]), "v"(byte[i]));
+      }
+    }
   }
   if (!live) return;
-  if (!is_v && (is_q || p.kn)) {
-    if (bad_slot) yw = u32x4_t{nan2, nan2, nan2, nan2};
-    uint16_t *dst = is_q ? p.qn : p.kn;
-    const uint32_t nh = is_q ? p.hq : p.hk;
-    st16_nt(dst + (((int64_t)b * nh + h) * p.S + s) * D + lc * 8, yw);
+  if (is_q || (p.kn && !is_v)) {
+    uint16_t *dst = (is_q ? p.qn : p.kn) + ((int64_t)(b * nh + h0) * p.S + s) * D + lc * 8;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (h0 + i < nh)
+        st16_nt(dst + (int64_t)i * p.S * D, bad_slot ? u32x4_t{nan2, nan2, nan2, nan2} : held[i]);
   }
   if (is_q || slot < 0 || bad_slot) return;
   const int64_t page = slot >> p.page_shift, at = slot & p.page_mask;
-  const int64_t off = page * p.cs[0] + h * p.cs[1] + at * p.cs[2] + lc * 8;
-  char *cache = is_v ? p.v_cache : p.k_cache;
-  if constexpr (FP8) {
-    *reinterpret_cast<u32x2_t *>(cache + off) = payload;
-    if (lc == 0) (is_v ? p.v_scale : p.k_scale)[page * p.es[0] + h * p.es[1] + at] = (uint8_t)byte;
-  } else {
-    st16(reinterpret_cast<uint16_t *>(cache) + off, held);
+  const int64_t off = page * p.cs[0] + h0 * p.cs[1] + at * p.cs[2] + lc * 8;
+  char *cache = (is_v ? p.v_cache : p.k_cache) + off * (FP8 ? 1 : 2);
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    if (h0 + i >= nh) break;
+    if constexpr (FP8) {
+      __builtin_nontemporal_store(payload[i], reinterpret_cast<u32x2_t *>(cache + i * p.cs[1]));
+      if (lc == 0) (is_v ? p.v_scale : p.k_scale)[page * p.es[0] + (h0 + i) * p.es[1] + at] = (uint8_t)byte[i];
+    } else {
+      st16_nt(reinterpret_cast<uint16_t *>(cache) + i * p.cs[1], held[i]);
+    }
   }
 }
 
-template <int D, int ST, bool ROPE, bool FP8>
+template <int D, int ST, bool ROPE, bool FP8, int U>
 hipError_t launch_write_t(const WriteParams &p, hipStream_t stream) {
-  const int64_t grid = ((int64_t)p.rows + 256 / (D / 8) - 1) / (256 / (D / 8));
-  hipLaunchKernelGGL((cache_write_kernel<D, ST, ROPE, FP8>), dim3((unsigned)grid), dim3(256), 0, stream, p);
+  constexpr uint32_t tokens = 256 / (D / 8);
+  const dim3 grid((p.T + tokens - 1) / tokens, (p.hq + U - 1) / U + 2 * ((p.hk + U - 1) / U));
+  hipLaunchKernelGGL((cache_write_kernel<D, ST, ROPE, FP8, U>), grid, dim3(256), 0, stream, p);
   static const std::string name = [] {
     char b[96];
-    snprintf(b, sizeof(b), "cache_write_kernel<%d, %d, %s, %s>", D, ST, tf(ROPE), tf(FP8));
+    snprintf(b, sizeof(b), "cache_write_kernel<%d, %d, %s, %s, %d>", D, ST, tf(ROPE), tf(FP8), U);
     return std::string(b);
   }();
-  launch_log_add(reinterpret_cast<const void *>(&cache_write_kernel<D, ST, ROPE, FP8>), name.c_str(), grid, 256);
+  launch_log_add(reinterpret_cast<const void *>(&cache_write_kernel<D, ST, ROPE, FP8, U>), name.c_str(),
+                 (int64_t)grid.x * grid.y, 256);
   return hipGetLastError();
+}
+
+template <int D, int ST, bool ROPE, bool FP8>
+hipError_t launch_write_u(const WriteParams &p, hipStream_t stream) {
+  const int64_t rows = (int64_t)p.T * (p.hq + 2 * p.hk);
+  return rows >= WIDE_ROWS ? launch_write_t<D, ST, ROPE, FP8, 4>(p, stream) : launch_write_t<D, ST, ROPE, FP8, 1>(p, stream);
 }
 
 template <int D, int ST>
 hipError_t dispatch_write(const WriteParams &p, bool rope, bool fp8, hipStream_t s) {
-  if (rope) return fp8 ? launch_write_t<D, ST, true, true>(p, s) : launch_write_t<D, ST, true, false>(p, s);
-  return fp8 ? launch_write_t<D, ST, false, true>(p, s) : launch_write_t<D, ST, false, false>(p, s);
+  if (rope) return fp8 ? launch_write_u<D, ST, true, true>(p, s) : launch_write_u<D, ST, true, false>(p, s);
+  return fp8 ? launch_write_u<D, ST, false, true>(p, s) : launch_write_u<D, ST, false, false>(p, s);
 }
 
 struct ReadParams {
@@ -171,64 +216,93 @@ struct ReadParams {
   uint16_t *k, *v;
   int64_t cs[3], es[2];
   int64_t pages_stride, lengths_stride, num_pages, capacity;
-  uint32_t L, hk, rows_per_seq;  // hk * L
+  uint32_t L, hk;
   int page_shift, page_mask;
   bool pages64, len64;
 };
 
-// One row of K and of V per LPR lanes: row (h, j) of sequence blockIdx.y.
-template <int D, bool FP8>
+// U times 256 / LPR rows of K and V of head blockIdx.y of sequence blockIdx.z
+// per workgroup; all of a lane's loads are issued before the first is waited for.
+template <int D, bool FP8, int U>
 __global__ __launch_bounds__(256) void cache_read_kernel(ReadParams p) {
-  constexpr int LPR = D / 8;
-  const int64_t b = blockIdx.y;
-  const uint32_t row = blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  const uint32_t lc = threadIdx.x % LPR;
-  if (row >= p.rows_per_seq) return;
-  const uint32_t h = row / p.L, j = row - h * p.L;
+  constexpr int LPR = D / 8, RPB = 256 / LPR;
+  const int64_t b = blockIdx.z, h = blockIdx.y;
+  const uint32_t lc = threadIdx.x % LPR, j0 = blockIdx.x * (RPB * U) + threadIdx.x / LPR;
   const int64_t len = load_index(p.lengths, p.len64, b * p.lengths_stride);
-  const uint32_t nan2 = 0x7fc07fc0u;
-  u32x4_t out[2] = {{0u, 0u, 0u, 0u}, {0u, 0u, 0u, 0u}};
-  bool bad = len < 0 || len > p.capacity;
-  if (!bad && j < len) {
-    const int64_t page = load_index(p.pages, p.pages64, b * p.pages_stride + (j >> p.page_shift));
-    bad = page < 0 || page >= p.num_pages;
-    if (!bad) {
-      const int64_t at = j & p.page_mask;
-      const int64_t off = page * p.cs[0] + h * p.cs[1] + at * p.cs[2] + lc * 8;
+  const bool bad_len = len < 0 || len > p.capacity;
+  int64_t page[U];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const char *c = i ? p.v_cache : p.k_cache;
-        if constexpr (FP8) {
-          const u32x2_t w = *reinterpret_cast<const u32x2_t *>(c + off);
-          const float sc = scale_value((i ? p.v_scale : p.k_scale)[page * p.es[0] + h * p.es[1] + at]);
-          float f[8];
-          unpack_e4m3(w, f);
+  for (int i = 0; i < U; ++i) {
+    const int64_t j = j0 + i * RPB;
+    page[i] = -2;  // nothing there
+    if (!bad_len && j < len && j < p.L) {
+      page[i] = load_index(p.pages, p.pages64, b * p.pages_stride + (j >> p.page_shift));
+      if (page[i] < 0 || page[i] >= p.num_pages) page[i] = -1;
+    }
+    if (bad_len) page[i] = -1;
+  }
+  u32x4_t raw[U][2];
+  float sc[U][2];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] *= sc;
-          out[i] = pack8(f);
-        } else {
-          out[i] = ld16(reinterpret_cast<const uint16_t *>(c) + off);
-        }
+  for (int i = 0; i < U; ++i) {
+    raw[i][0] = raw[i][1] = u32x4_t{0u, 0u, 0u, 0u};
+    sc[i][0] = sc[i][1] = 1.0f;
+    if (page[i] < 0) continue;
+    const int64_t at = (j0 + i * RPB) & p.page_mask;
+    const int64_t off = page[i] * p.cs[0] + h * p.cs[1] + at * p.cs[2] + lc * 8;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const char *c = x ? p.v_cache : p.k_cache;
+      if constexpr (FP8) {
+        const u32x2_t w = __builtin_nontemporal_load(reinterpret_cast<const u32x2_t *>(c + off));
+        raw[i][x][0] = w[0];
+        raw[i][x][1] = w[1];
+        sc[i][x] = scale_value((x ? p.v_scale : p.k_scale)[page[i] * p.es[0] + h * p.es[1] + at]);
+      } else {
+        raw[i][x] = ld16_nt(reinterpret_cast<const uint16_t *>(c) + off);
       }
     }
   }
-  if (bad) out[0] = out[1] = u32x4_t{nan2, nan2, nan2, nan2};
-  const int64_t o = (b * p.rows_per_seq + row) * D + lc * 8;
-  st16_nt(p.k + o, out[0]);
-  st16_nt(p.v + o, out[1]);
+  const uint32_t nan2 = 0x7fc07fc0u;
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const uint32_t j = j0 + i * RPB;
+    if (j >= p.L) break;
+    const int64_t o = (((int64_t)b * p.hk + h) * p.L + j) * D + lc * 8;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      u32x4_t out = raw[i][x];
+      if constexpr (FP8) {
+        float f[8];
+        unpack_e4m3(u32x2_t{out[0], out[1]}, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= sc[i][x];
+        out = pack8(f);
+      }
+      if (page[i] == -1) out = u32x4_t{nan2, nan2, nan2, nan2};
+      st16_nt((x ? p.v : p.k) + o, out);
+    }
+  }
+}
+
+template <int D, bool FP8, int U>
+hipError_t launch_read_t(const ReadParams &p, int64_t B, hipStream_t stream) {
+  constexpr uint32_t rows = 256 / (D / 8) * U;
+  const dim3 grid((p.L + rows - 1) / rows, p.hk, (unsigned)B);
+  hipLaunchKernelGGL((cache_read_kernel<D, FP8, U>), grid, dim3(256), 0, stream, p);
+  static const std::string name = [] {
+    char b[96];
+    snprintf(b, sizeof(b), "cache_read_kernel<%d, %s, %d>", D, tf(FP8), U);
+    return std::string(b);
+  }();
+  launch_log_add(reinterpret_cast<const void *>(&cache_read_kernel<D, FP8, U>), name.c_str(),
+                 (int64_t)grid.x * grid.y * grid.z, 256);
+  return hipGetLastError();
 }
 
 template <int D, bool FP8>
-hipError_t launch_read_t(const ReadParams &p, int64_t B, hipStream_t stream) {
-  const dim3 grid((p.rows_per_seq + 256 / (D / 8) - 1) / (256 / (D / 8)), (unsigned)B);
-  hipLaunchKernelGGL((cache_read_kernel<D, FP8>), grid, dim3(256), 0, stream, p);
-  static const std::string name = [] {
-    char b[96];
-    snprintf(b, sizeof(b), "cache_read_kernel<%d, %s>", D, tf(FP8));
-    return std::string(b);
-  }();
-  launch_log_add(reinterpret_cast<const void *>(&cache_read_kernel<D, FP8>), name.c_str(), (int64_t)grid.x * grid.y, 256);
-  return hipGetLastError();
+hipError_t launch_read_u(const ReadParams &p, int64_t B, hipStream_t stream) {
+  return B * p.hk * p.L >= WIDE_ROWS ? launch_read_t<D, FP8, 4>(p, B, stream) : launch_read_t<D, FP8, 1>(p, B, stream);
 }
 
 }  // namespace
@@ -252,7 +326,6 @@ hipError_t launch_cache_write(const kfmi_cache_write_args &a, int style, hipStre
   p.T = (uint32_t)(a.B * a.S);
   p.hq = a.q ? (uint32_t)a.Hq : 0u;
   p.hk = (uint32_t)a.Hkv;
-  p.rows = p.T * (p.hq + 2 * p.hk);
   p.table_rows = a.table_rows;
   p.slot_end = a.num_pages * a.page_size;
   p.page_shift = log2_of(a.page_size);
@@ -289,14 +362,13 @@ hipError_t launch_cache_read(const kfmi_cache_read_args &a, hipStream_t stream) 
   p.capacity = a.max_pages * a.page_size;
   p.L = (uint32_t)a.L;
   p.hk = (uint32_t)a.Hkv;
-  p.rows_per_seq = p.hk * p.L;
   p.page_shift = log2_of(a.page_size);
   p.page_mask = (int)(a.page_size - 1);
   p.pages64 = a.index_flags & KFMI_I64_PAGES;
   p.len64 = a.index_flags & KFMI_I64_LENGTHS;
   const bool fp8 = a.cache_type == KFMI_CACHE_E4M3;
-  if (a.D == 128) return fp8 ? launch_read_t<128, true>(p, a.B, stream) : launch_read_t<128, false>(p, a.B, stream);
-  return fp8 ? launch_read_t<256, true>(p, a.B, stream) : launch_read_t<256, false>(p, a.B, stream);
+  if (a.D == 128) return fp8 ? launch_read_u<128, true>(p, a.B, stream) : launch_read_u<128, false>(p, a.B, stream);
+  return fp8 ? launch_read_u<256, true>(p, a.B, stream) : launch_read_u<256, false>(p, a.B, stream);
 }
 
 }  // namespace kfmi

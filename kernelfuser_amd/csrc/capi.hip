@@ -522,6 +522,7 @@ static int check_cache(const void *k, const void *v, const void *ks, const void 
 int kfmi_norm_rope_to_cache_bf16(const kfmi_cache_write_args *a, void *stream) {
   if (a == nullptr) return fail(KFMI_EINVAL, "args must not be NULL");
   KFMI_TRY(check_sizes(a->B, a->q ? a->Hq : a->Hkv, a->Hkv, a->S, a->D));
+  if ((a->q ? a->Hq : 0) + 2 * a->Hkv > 65535) return fail(KFMI_EINVAL, "Hq + 2 * Hkv must be at most 65535");
   KFMI_TRY(check_style(a->norm_style));
   if (a->index_flags & ~(KFMI_I64_POSITIONS | KFMI_I64_SLOTS)) return fail(KFMI_EINVAL, "unknown index_flags 0x%x", a->index_flags);
   KFMI_TRY(check_ptrs({{a->k, "k"}, {a->v, "v"}, {a->gk, "gk"}}));
@@ -590,6 +591,7 @@ int kfmi_cache_to_dense_bf16(const kfmi_cache_read_args *a, void *stream) {
   if (a == nullptr) return fail(KFMI_EINVAL, "args must not be NULL");
   KFMI_TRY(check_sizes(a->B, a->Hkv, a->Hkv, a->L, a->D));
   if (a->B > 65535) return fail(KFMI_EINVAL, "B must be at most 65535 (got %lld)", (long long)a->B);
+  if (a->Hkv > 65535) return fail(KFMI_EINVAL, "Hkv must be at most 65535 (got %lld)", (long long)a->Hkv);
   if (a->max_pages < 1) return fail(KFMI_EINVAL, "max_pages must be >= 1 (got %lld)", (long long)a->max_pages);
   if (a->index_flags & ~(KFMI_I64_PAGES | KFMI_I64_LENGTHS)) return fail(KFMI_EINVAL, "unknown index_flags 0x%x", a->index_flags);
   KFMI_TRY(check_index(a->pages, a->index_flags, KFMI_I64_PAGES, "pages"));

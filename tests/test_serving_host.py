@@ -119,6 +119,7 @@ WRITE, DECODE, READ, LOGPROBS = ("kfmi_norm_rope_to_cache_bf16", "kfmi_attention
 REFUSED = [
     (WRITE, _write, dict(B=0), ">= 1"), (WRITE, _write, dict(D=64), "D must be"),
     (WRITE, _write, dict(Hq=7), "multiple of Hkv"), (WRITE, _write, dict(style=5), "norm_style"),
+    (WRITE, _write, dict(B=1, Hq=2 ** 16, Hkv=2 ** 16), "65535"), (READ, _read, dict(B=1, Hkv=2 ** 16), "65535"),
     (WRITE, _write, dict(B=2 ** 20, S=2 ** 12), "2^31"), (WRITE, _write, dict(B=2 ** 40, S=2 ** 40), "2^31"),
     (WRITE, _write, dict(flags=4), "index_flags"), (WRITE, _write, dict(k=0), "k must not"),
     (WRITE, _write, dict(qn=0), "qn must not"), (WRITE, _write, dict(v=P + 8), "v must be 16"),
