@@ -29,9 +29,9 @@ import torch
 
 from . import _lib
 from ._lib import NORM_STYLES
-from .ops import EPS, _on_device, device_arch
+from .ops import EPS, device_arch
 
-_I32, _I64 = torch.int32, torch.int64
+_I32, _I64, _F32 = torch.int32, torch.int64, torch.float32
 _BF16, _E4M3, _E8M0 = torch.bfloat16, torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
@@ -55,17 +55,45 @@ def make_cache(pages: int, hkv: int, page_size: int, d: int, dtype=torch.bfloat1
 # Checks
 # ---------------------------------------------------------------------------
 
-def _check_gpu(tensors, device):
-    if device.type != "cuda":
-        raise ValueError("Inputs must be on one GPU device")
+# The checks read each property once and without helper objects: an eager call
+# of one token is bound by them, not by its kernel (a property costs 70 to 160 ns).
+
+_checked_devices: set[int] = set()
+
+
+def _check_gpu(index, *tensors):
+    """All tensors on the gfx950 device of this index (-1: the CPU)."""
     for t in tensors:
-        if t.device != device:
+        if t is not None and t.get_device() != index:
             raise ValueError("Inputs must be on one GPU device")
-    if not device_arch(device).startswith("gfx950"):
-        raise ValueError(f"This implementation targets gfx950 (MI355X); device is {device_arch(device)}")
+    if index not in _checked_devices:
+        if index < 0:
+            raise ValueError("Inputs must be on one GPU device")
+        arch = device_arch(torch.device("cuda", index))
+        if not arch.startswith("gfx950"):
+            raise ValueError(f"This implementation targets gfx950 (MI355X); device is {arch}")
+        _checked_devices.add(index)
 
 
-def _check_grad(tensors, name):
+def _call(index, entry, packed, work=None):
+    """One entry point on the current stream of the device.  ``work``: a function of the stream that
+    gives (address, bytes, tensor) of the workspace, whose place in ``packed`` it fills."""
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(index):
+            return _call(index, entry, packed, work)
+    stream = _raw_stream(index)
+    if work is not None:
+        wp, wb, buf = work(stream)
+        packed = packed(wp, wb)
+    _lib.call(entry, packed, stream)
+
+
+def _raw_stream(index):
+    raw = _lib._raw_stream
+    return torch.cuda.current_stream(index).cuda_stream if raw is None else raw(index)
+
+
+def _check_grad(name, *tensors):
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -125,45 +153,41 @@ def _row_strides(t, name):
 
 COUNTER_BYTES = 8192  # KFMI_DECODE_COUNTER_BYTES, KFMI_LOGPROBS_COUNTER_BYTES
 
-_work_cache: dict[tuple[int, int], torch.Tensor] = {}
+_work_cache: dict[tuple[int, int], tuple[int, int, torch.Tensor]] = {}
 _work_retired: list[torch.Tensor] = []
 _size_cache: dict[tuple, int] = {}
 
 
-def _workspace_bytes(entry, key, packed):
-    """Bytes that a workspace query answers for these arguments, asked once per (device, sizes)."""
-    key = (entry, torch.cuda.current_device() if torch.cuda.is_available() else -1) + key
-    n = _size_cache.get(key)
-    if n is None:
-        got = ctypes.c_int64()
-        lib = _lib.load()
-        if getattr(lib, entry)(packed, ctypes.byref(got)) != _lib.KFMI_OK:
-            raise ValueError(f"{entry}: {lib.kfmi_last_error().decode(errors='replace')}")
-        n = _size_cache[key] = got.value
-    return n
+def _ask_workspace(entry, packed):
+    """Bytes that a workspace query answers for these arguments."""
+    got = ctypes.c_int64()
+    lib = _lib.load()
+    if getattr(lib, entry)(packed, ctypes.byref(got)) != _lib.KFMI_OK:
+        raise ValueError(f"{entry}: {lib.kfmi_last_error().decode(errors='replace')}")
+    return got.value
 
 
-def _workspace(device, stream, nbytes):
+def _workspace(index, stream, nbytes):
     """(address, bytes, tensor) of a workspace with zeroed counters for a launch
-    on ``stream`` of the current device."""
+    on ``stream`` of the current device ``index``."""
     if nbytes <= 0:
         return 0, 0, None
     if torch.cuda.is_current_stream_capturing():
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=index)
         buf[:COUNTER_BYTES].zero_()  # a fill kernel inside the graph, not a memset node
         return buf.data_ptr(), nbytes, buf
-    key = (device.index, stream)
+    key = (index, stream)
     buf = _work_cache.get(key)
-    if buf is None or buf.numel() < nbytes:
+    if buf is None or buf[1] < nbytes:
         if buf is not None:
-            _work_retired.append(buf)  # launches that hold its address may still run
-        buf = torch.zeros(max(nbytes, 0 if buf is None else 2 * buf.numel()), dtype=torch.uint8, device=device)
-        _work_cache[key] = buf
-    return buf.data_ptr(), buf.numel(), buf
+            _work_retired.append(buf[2])  # launches that hold its address may still run
+        t = torch.zeros(max(nbytes, 0 if buf is None else 2 * buf[1]), dtype=torch.uint8, device=index)
+        buf = _work_cache[key] = (t.data_ptr(), t.numel(), t)
+    return buf
 
 
-def _given_work(work, device):
-    if work.device != device or not work.is_contiguous():
+def _given_work(work, index):
+    if work.get_device() != index or not work.is_contiguous():
         raise ValueError("work must be a contiguous tensor on the inputs' device")
     return work.data_ptr(), work.numel() * work.element_size(), work
 
@@ -192,82 +216,97 @@ def norm_rope_to_cache(q, k, v, gq, gk, cos, sin, positions, slots, k_cache, v_c
     A position outside the tables makes its token's rows of ``qn``, ``kn`` and
     the cached K NaN; a slot behind the cache makes its rows of ``qn`` and ``kn`` NaN and is not written.
     """
-    if norm_style not in NORM_STYLES:
+    style = NORM_STYLES.get(norm_style)
+    if style is None:
         raise ValueError("norm_style must be 'hf', 'legacy' or 'fp32'")
     if (cos is None) != (sin is None):
         raise ValueError("Pass both rotary tables (cos and sin) or neither")
-    rows = (k, v, gk) if q is None else (q, k, v, gq, gk)
-    if any(t is None for t in rows):
+    if k is None or v is None or gk is None or (q is not None and gq is None):
         raise ValueError("Expected k, v and gk (and gq with q)")
-    tables = () if cos is None else (cos, sin)
-    _check_grad(rows + tables, "norm_rope_to_cache")
-    if k.ndim != 4 or k.shape != v.shape:
+    _check_grad("norm_rope_to_cache", q, k, v, gq, gk, cos, sin)
+    shape, d1 = k.shape, (k.shape[-1],)
+    if len(shape) != 4 or v.shape != shape:
         raise ValueError("Expected q [B,Hq,S,D] and k, v [B,Hkv,S,D]")
-    b, hk, s, d = k.shape
-    hq = 0
-    if q is not None:
-        if q.ndim != 4 or q.shape[0] != b or q.shape[2] != s or q.shape[3] != d:
-            raise ValueError("Expected q [B,Hq,S,D] and k, v [B,Hkv,S,D]")
-        hq = q.shape[1]
-    if d not in (128, 256) or min(b, hk, s) < 1 or (q is not None and (hq < 1 or hq % hk)):
+    b, hk, s, d = shape
+    if d not in (128, 256) or b < 1 or hk < 1 or s < 1:
         raise ValueError("Expected D in (128, 256), B, S >= 1 and Hq a multiple of Hkv")
-    for t in rows + tables:
-        if t.dtype is not _BF16:
-            raise ValueError("Inputs must be BF16 tensors")
-    if gk.shape != (d,) or (q is not None and gq.shape != (d,)):
+    if k.dtype is not _BF16 or v.dtype is not _BF16 or gk.dtype is not _BF16:
+        raise ValueError("Inputs must be BF16 tensors")
+    if gk.shape != d1:
         raise ValueError("Expected gamma vectors [D]")
+    ks, vs = _row_strides(k, "k"), _row_strides(v, "v")
+    index = k.get_device()
+    hq, qs, q_ptr, gq_ptr = 0, (0, 0, 0), 0, 0
+    if q is not None:
+        qshape = q.shape
+        if len(qshape) != 4 or qshape[0] != b or qshape[2] != s or qshape[3] != d:
+            raise ValueError("Expected q [B,Hq,S,D] and k, v [B,Hkv,S,D]")
+        hq = qshape[1]
+        if hq < 1 or hq % hk:
+            raise ValueError("Expected D in (128, 256), B, S >= 1 and Hq a multiple of Hkv")
+        if q.dtype is not _BF16 or gq.dtype is not _BF16:
+            raise ValueError("Inputs must be BF16 tensors")
+        if gq.shape != d1:
+            raise ValueError("Expected gamma vectors [D]")
+        if not gq.is_contiguous():
+            raise ValueError("gamma vectors and rotary tables must be contiguous")
+        qs, q_ptr, gq_ptr = _row_strides(q, "q"), q.data_ptr(), gq.data_ptr()
     flags = _wide(slots, _lib.I64_SLOTS, "slots")
     if slots.shape != (b, s):
         raise ValueError("Expected slots [B,S]")
-    table_rows, pos_ptr, pos_strides, pos = 0, None, (0, 0), ()
+    table_rows, cos_ptr, sin_ptr, pos_ptr, pos_strides = 0, 0, 0, 0, (0, 0)
     if cos is not None:
         if positions is None or positions.shape != (b, s):
             raise ValueError("Expected positions [B,S] with rotary tables")
-        if cos.ndim != 2 or cos.shape[1] != d or cos.shape != sin.shape or cos.shape[0] < 1:
+        tshape = cos.shape
+        if len(tshape) != 2 or tshape[1] != d or sin.shape != tshape or tshape[0] < 1:
             raise ValueError("Expected rotary tables [P,D]")
-        flags |= _wide(positions, _lib.I64_POSITIONS, "positions")
-        table_rows, pos_ptr, pos_strides, pos = cos.shape[0], positions.data_ptr(), positions.stride(), (positions,)
-    for t in (gk, *tables) if q is None else (gq, gk, *tables):
-        if not t.is_contiguous():
+        if cos.dtype is not _BF16 or sin.dtype is not _BF16:
+            raise ValueError("Inputs must be BF16 tensors")
+        if not cos.is_contiguous() or not sin.is_contiguous():
             raise ValueError("gamma vectors and rotary tables must be contiguous")
-    shape, cs, es, kind = _check_cache(k_cache, v_cache, k_scale, v_scale)
-    if shape[1] != hk or shape[3] != d:
+        flags |= _wide(positions, _lib.I64_POSITIONS, "positions")
+        table_rows, cos_ptr, sin_ptr = tshape[0], cos.data_ptr(), sin.data_ptr()
+        pos_ptr, pos_strides = positions.data_ptr(), positions.stride()
+    if not gk.is_contiguous():
+        raise ValueError("gamma vectors and rotary tables must be contiguous")
+    cshape, cs, es, kind = _check_cache(k_cache, v_cache, k_scale, v_scale)
+    if cshape[1] != hk or cshape[3] != d:
         raise ValueError("The cache's Hkv and D must be those of k and v")
-    qs = (0, 0, 0) if q is None else _row_strides(q, "q")
-    ks, vs = _row_strides(k, "k"), _row_strides(v, "v")
     if b * s * max(hq, hk) * d >= 2 ** 31:
         raise ValueError("Tensors must have fewer than 2**31 elements")
-    outs = ()
-    for name, out, like in (("qn", qn, q), ("kn", kn, k)):
-        if out is not None:
-            if like is None or out.shape != like.shape or out.dtype is not _BF16 or not out.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous BF16 tensor shaped like its input on the same device")
-            outs += (out,)
-    scales = () if k_scale is None else (k_scale, v_scale)
-    device = k.device
-    _check_gpu((*rows, *tables, slots, *pos, k_cache, v_cache, *scales, *outs), device)
-    if not float(eps) >= 0.0:
+    if qn is not None:
+        _check_out("qn", qn, None if q is None else qshape)
+    if kn is not None:
+        _check_out("kn", kn, shape)
+    _check_gpu(index, q, v, gq if q is not None else None, gk, cos, sin, positions if cos is not None else None, slots,
+               k_cache, v_cache, k_scale, v_scale, qn, kn)
+    if not eps >= 0.0:
         raise ValueError("eps must be >= 0")
     if q is not None and qn is None:
-        qn = torch.empty(q.shape, dtype=_BF16, device=device)
-    with _on_device(device):
-        _lib.call("kfmi_norm_rope_to_cache_bf16", _lib.CACHE_WRITE_ARGS.pack(
-            0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), 0 if q is None else gq.data_ptr(),
-            gk.data_ptr(), 0 if cos is None else cos.data_ptr(), 0 if cos is None else sin.data_ptr(), pos_ptr or 0,
-            slots.data_ptr(), 0 if q is None else qn.data_ptr(), 0 if kn is None else kn.data_ptr(),
-            k_cache.data_ptr(), v_cache.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
-            0 if v_scale is None else v_scale.data_ptr(), *qs, *ks, *vs,
-            *pos_strides, *slots.stride(), *cs[:3], *es, b, hq, hk, s, d, table_rows, shape[0], shape[2],
-            float(eps), NORM_STYLES[norm_style], kind, flags, 0), _lib.stream_of(k))
+        qn = torch.empty(qshape, dtype=_BF16, device=index)
+    _call(index, "kfmi_norm_rope_to_cache_bf16", _lib.CACHE_WRITE_ARGS.pack(
+        q_ptr, k.data_ptr(), v.data_ptr(), gq_ptr, gk.data_ptr(), cos_ptr, sin_ptr, pos_ptr, slots.data_ptr(),
+        0 if q is None else qn.data_ptr(), 0 if kn is None else kn.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+        0 if k_scale is None else k_scale.data_ptr(), 0 if k_scale is None else v_scale.data_ptr(), *qs, *ks, *vs,
+        *pos_strides, *slots.stride(), cs[0], cs[1], cs[2], *es, b, hq, hk, s, d, table_rows, cshape[0], cshape[2],
+        eps, style, kind, flags, 0))
     return qn
 
 
+def _check_out(name, out, shape):
+    if shape is None or out.shape != shape or out.dtype is not _BF16 or not out.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous BF16 tensor shaped like its input on the same device")
+
+
 def _pages_and_lengths(pages, lengths, b):
-    if pages.ndim != 2 or pages.shape[0] != b or pages.shape[1] < 1 or pages.stride(1) != 1:
+    """Their index flags, the pages per sequence and the stride between them."""
+    shape, stride = pages.shape, pages.stride()
+    if len(shape) != 2 or shape[0] != b or shape[1] < 1 or stride[1] != 1:
         raise ValueError("Expected pages [B,max_pages] with contiguous rows")
     if lengths.shape != (b,):
         raise ValueError("Expected lengths [B]")
-    return _wide(pages, _lib.I64_PAGES, "pages") | _wide(lengths, _lib.I64_LENGTHS, "lengths")
+    return (_wide(pages, _lib.I64_PAGES, "pages") | _wide(lengths, _lib.I64_LENGTHS, "lengths"), shape[1], stride[0])
 
 
 def cache_to_dense(k_cache, v_cache, pages, lengths, max_length, k_scale=None, v_scale=None, *, k=None, v=None):
@@ -280,29 +319,25 @@ def cache_to_dense(k_cache, v_cache, pages, lengths, max_length, k_scale=None, v
     shape, cs, es, kind = _check_cache(k_cache, v_cache, k_scale, v_scale)
     num_pages, hk, page, d = shape
     b, l = lengths.shape[0] if lengths.ndim == 1 else 0, int(max_length)
-    flags = _pages_and_lengths(pages, lengths, b)
+    flags, _, _ = _pages_and_lengths(pages, lengths, b)
     if b < 1 or l < 1:
         raise ValueError("Expected B and max_length >= 1")
     if b * hk * l * d >= 2 ** 31:
         raise ValueError("Tensors must have fewer than 2**31 elements")
-    outs = ()
     for name, out in (("k", k), ("v", v)):
-        if out is not None:
-            if out.shape != (b, hk, l, d) or out.dtype is not _BF16 or not out.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous BF16 tensor [B,Hkv,max_length,D]")
-            outs += (out,)
-    device = k_cache.device
-    _check_gpu((v_cache, pages, lengths, *outs, *(() if k_scale is None else (k_scale, v_scale))), device)
+        if out is not None and (out.shape != (b, hk, l, d) or out.dtype is not _BF16 or not out.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous BF16 tensor [B,Hkv,max_length,D]")
+    index = k_cache.get_device()
+    _check_gpu(index, v_cache, pages, lengths, k, v, k_scale, v_scale)
     if k is None:
-        k = torch.empty(b, hk, l, d, dtype=_BF16, device=device)
+        k = torch.empty((b, hk, l, d), dtype=_BF16, device=index)
     if v is None:
-        v = torch.empty(b, hk, l, d, dtype=_BF16, device=device)
-    with _on_device(device):
-        _lib.call("kfmi_cache_to_dense_bf16", _lib.CACHE_READ_ARGS.pack(
-            k_cache.data_ptr(), v_cache.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
-            0 if v_scale is None else v_scale.data_ptr(), pages.data_ptr(), lengths.data_ptr(), k.data_ptr(),
-            v.data_ptr(), *cs[:3], *es, pages.stride(0), lengths.stride(0), b, hk, l, d, num_pages, page,
-            pages.shape[1], kind, flags), _lib.stream_of(k_cache))
+        v = torch.empty((b, hk, l, d), dtype=_BF16, device=index)
+    _call(index, "kfmi_cache_to_dense_bf16", _lib.CACHE_READ_ARGS.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
+        0 if v_scale is None else v_scale.data_ptr(), pages.data_ptr(), lengths.data_ptr(), k.data_ptr(),
+        v.data_ptr(), cs[0], cs[1], cs[2], *es, pages.stride(0), lengths.stride(0), b, hk, l, d, num_pages, page,
+        pages.shape[1], kind, flags))
     return k, v
 
 
@@ -334,58 +369,64 @@ def attention_decode(q, k_cache, v_cache, pages, lengths, k_scale=None, v_scale=
     graph is captured, one of the graph's own, zeroed on each replay.  The
     result's bits depend on the lengths in the batch, not on timing.
     """
-    _check_grad((q,), "attention_decode")
-    if q.ndim != 4 or q.dtype is not _BF16:
+    _check_grad("attention_decode", q)
+    qshape = q.shape
+    if len(qshape) != 4 or q.dtype is not _BF16:
         raise ValueError("Expected q [B,Hq,S,D] in BF16")
-    b, hq, s, d = q.shape
+    b, hq, s, d = qshape
     shape, cs, es, kind = _check_cache(k_cache, v_cache, k_scale, v_scale)
     num_pages, hk, page, cd = shape
-    if d != cd or min(b, hq, s) < 1 or hq % hk:
+    if d != cd or b < 1 or hq < 1 or s < 1 or hq % hk:
         raise ValueError("Expected the cache's D and Hq a multiple of its Hkv")
     if s > 16:
         raise ValueError("attention_decode takes at most 16 tokens per sequence")
-    flags = _pages_and_lengths(pages, lengths, b)
-    if window is not None and int(window) < 1:
+    flags, max_pages, pages_stride = _pages_and_lengths(pages, lengths, b)
+    if window is None:
+        window = 0
+    elif int(window) < 1:
         raise ValueError("window must be >= 1")
-    if softcap is not None and not 0.0 < float(softcap) < float("inf"):
+    if softcap is None:
+        softcap = 0.0
+    elif not 0.0 < softcap < float("inf"):
         raise ValueError("softcap must be positive and finite")
-    if scale is not None and not 0.0 < float(scale) < float("inf"):
+    if scale is None:
+        scale = d ** -0.5
+    elif not 0.0 < scale < float("inf"):
         raise ValueError("scale must be positive and finite")
     if b * hq * s * d >= 2 ** 31:
         raise ValueError("Tensors must have fewer than 2**31 elements")
-    if out is not None and (out.shape != q.shape or out.dtype is not _BF16 or not out.is_contiguous()):
+    if out is not None and (out.shape != qshape or out.dtype is not _BF16 or not out.is_contiguous()):
         raise ValueError("out must be a contiguous BF16 tensor shaped like q")
     qs = _row_strides(q, "q")
-    device = q.device
-    extra = () if k_scale is None else (k_scale, v_scale)
-    _check_gpu((k_cache, v_cache, pages, lengths, *extra, *(() if out is None else (out,))), device)
+    index = q.get_device()
+    _check_gpu(index, k_cache, v_cache, pages, lengths, k_scale, v_scale, out)
     if out is None:
-        out = torch.empty((b, hq, s, d), dtype=_BF16, device=device)
-    with _on_device(device):
-        stream = _lib.stream_of(q)
-        if work is None:
-            wp, wb, buf = _workspace(device, stream, attention_decode_workspace_bytes(
-                b, hq, hk, s, d, pages.shape[1] * page))
-        else:
-            wp, wb, buf = _given_work(work, device)
-        _lib.call("kfmi_attention_decode_bf16", _lib.DECODE_ARGS.pack(
+        out = torch.empty(qshape, dtype=_BF16, device=index)
+
+    def space(stream):
+        if work is not None:
+            return _given_work(work, index)
+        return _workspace(index, stream, attention_decode_workspace_bytes(b, hq, hk, s, d, max_pages * page))
+
+    def packed(wp, wb):
+        return _lib.DECODE_ARGS.pack(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
-            0 if v_scale is None else v_scale.data_ptr(), pages.data_ptr(), lengths.data_ptr(), out.data_ptr(), wp,
-            wb, *qs, *cs[:3], *es, pages.stride(0), lengths.stride(0), b, hq, hk, s, d, num_pages, page,
-            pages.shape[1], 0 if window is None else int(window), d ** -0.5 if scale is None else float(scale),
-            0.0 if softcap is None else float(softcap), kind, flags), stream)
+            0 if k_scale is None else v_scale.data_ptr(), pages.data_ptr(), lengths.data_ptr(), out.data_ptr(), wp,
+            wb, *qs, cs[0], cs[1], cs[2], *es, pages_stride, lengths.stride(0), b, hq, hk, s, d, num_pages, page,
+            max_pages, int(window), scale, softcap, kind, flags)
+
+    _call(index, "kfmi_attention_decode_bf16", packed, space)
     return out
 
 
 def attention_decode_workspace_bytes(b: int, hq: int, hkv: int, s: int, d: int, max_keys: int) -> int:
-    """Bytes of ``attention_decode``'s workspace on the current device for sequences of up to ``max_keys``."""
+    """Bytes of ``attention_decode``'s workspace for sequences of up to ``max_keys``."""
     key = (b, hq, hkv, s, d, max_keys)
-    n = _size_cache.get(("d", torch.cuda.current_device() if torch.cuda.is_available() else -1) + key)
+    n = _size_cache.get(key)
     if n is None:
         pages = -(-max_keys // 16)
-        packed = _lib.DECODE_ARGS.pack(*[0] * 9, 0, *[0] * 8, 0, 0, b, hq, hkv, s, d, 1, 16, pages, 0, 1.0, 0.0, 0, 0)
-        n = _workspace_bytes("kfmi_attention_decode_workspace", key, packed)
-        _size_cache[("d", torch.cuda.current_device() if torch.cuda.is_available() else -1) + key] = n
+        n = _size_cache[key] = _ask_workspace("kfmi_attention_decode_workspace", _lib.DECODE_ARGS.pack(
+            *[0] * 9, 0, *[0] * 8, 0, 0, b, hq, hkv, s, d, 1, 16, pages, 0, 1.0, 0.0, 0, 0))
     return n
 
 
@@ -411,46 +452,52 @@ def token_logprobs(logits, ids, top=0, *, work=None) -> TokenLogprobs:
     nothing but -infinity, is no distribution: NaN everywhere and top_ids -1.
 
     ``work``: as for ``attention_decode`` (``token_logprobs_workspace_bytes``)."""
-    _check_grad((logits,), "token_logprobs")
+    _check_grad("token_logprobs", logits)
     kind = _lib.LOGITS_TYPES.get(logits.dtype)
     if kind is None:
         raise ValueError("logits must be float32, bfloat16 or float16")
-    lead = logits.shape[:-1]
-    if not 1 <= logits.ndim <= 3 or ids.shape != lead:
+    shape, ls, is_ = logits.shape, logits.stride(), ids.stride()
+    lead = shape[:-1]
+    if not 1 <= len(shape) <= 3 or ids.shape != lead:
         raise ValueError("Expected logits [...,V] with up to two leading dimensions and ids [...]")
     flags = _wide(ids, _lib.I64_IDS, "ids")
-    v, top = logits.shape[-1], int(top)
-    if v < 1 or v >= 2 ** 30 or (v > 1 and logits.stride(-1) != 1):
+    v, top = shape[-1], int(top)
+    if v < 1 or v >= 2 ** 30 or (v > 1 and ls[-1] != 1):
         raise ValueError("logits need contiguous rows of 1 to 2**30 - 1 values")
     if not 0 <= top <= min(_lib.LOGPROBS_TOP_MAX, v):
         raise ValueError(f"top must be from 0 to {_lib.LOGPROBS_TOP_MAX} and at most V")
     n0, n1 = (1, 1, *lead)[-2:]
     if n0 * n1 >= 2 ** 25:
         raise ValueError("Expected fewer than 2**25 rows")
-    device = logits.device
-    _check_gpu((ids,), device)
-    out = torch.empty(lead, dtype=torch.float32, device=device), torch.empty(lead, dtype=torch.float32, device=device)
+    index = logits.get_device()
+    _check_gpu(index, ids)
+    out, entropy = torch.empty((2, *lead), dtype=_F32, device=index).unbind(0)
     tops = (None, None)
     if top:
-        tops = (torch.empty(*lead, top, dtype=torch.float32, device=device),
-                torch.empty(*lead, top, dtype=_I64, device=device))
+        tops = (torch.empty((*lead, top), dtype=_F32, device=index), torch.empty((*lead, top), dtype=_I64, device=index))
     if n0 * n1 == 0:
-        return TokenLogprobs(*out, *tops)
-    with _on_device(device):
-        stream = _lib.stream_of(logits)
-        if work is None:
-            wp, wb, buf = _workspace(device, stream, token_logprobs_workspace_bytes(n0 * n1, v, top, logits.dtype))
-        else:
-            wp, wb, buf = _given_work(work, device)
-        _lib.call("kfmi_token_logprobs", _lib.LOGPROBS_ARGS.pack(
-            logits.data_ptr(), ids.data_ptr(), out[0].data_ptr(), out[1].data_ptr(),
-            tops[0].data_ptr() if top else 0, tops[1].data_ptr() if top else 0, wp, wb,
-            *(0, 0, *logits.stride()[:-1])[-2:], *(0, 0, *ids.stride())[-2:], n0, n1, v, top, kind, flags, 0), stream)
-    return TokenLogprobs(*out, *tops)
+        return TokenLogprobs(out, entropy, *tops)
+
+    def space(stream):
+        if work is not None:
+            return _given_work(work, index)
+        return _workspace(index, stream, token_logprobs_workspace_bytes(n0 * n1, v, top, logits.dtype))
+
+    def packed(wp, wb):
+        return _lib.LOGPROBS_ARGS.pack(
+            logits.data_ptr(), ids.data_ptr(), out.data_ptr(), entropy.data_ptr(), tops[0].data_ptr() if top else 0,
+            tops[1].data_ptr() if top else 0, wp, wb, *(0, 0, *ls[:-1])[-2:], *(0, 0, *is_)[-2:], n0, n1, v, top, kind,
+            flags, 0)
+
+    _call(index, "kfmi_token_logprobs", packed, space)
+    return TokenLogprobs(out, entropy, *tops)
 
 
 def token_logprobs_workspace_bytes(n: int, v: int, top: int, dtype=torch.float32) -> int:
-    """Bytes of ``token_logprobs``'s workspace on the current device for ``n`` rows of ``v`` logits."""
-    kind = _lib.LOGITS_TYPES[dtype]
-    return _workspace_bytes("kfmi_token_logprobs_workspace", (n, v, top, kind), _lib.LOGPROBS_ARGS.pack(
-        *[0] * 7, 0, 0, 0, 0, 0, 1, n, v, top, kind, 0, 0))
+    """Bytes of ``token_logprobs``'s workspace for ``n`` rows of ``v`` logits."""
+    key = (n, v, top, dtype)
+    size = _size_cache.get(key)
+    if size is None:
+        size = _size_cache[key] = _ask_workspace("kfmi_token_logprobs_workspace", _lib.LOGPROBS_ARGS.pack(
+            *[0] * 7, 0, 0, 0, 0, 0, 1, n, v, top, _lib.LOGITS_TYPES[dtype], 0, 0))
+    return size
