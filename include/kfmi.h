@@ -361,7 +361,7 @@ typedef struct {
   int64_t pages_stride, lengths_stride;      /* between sequences, in elements */
   int64_t B, Hq, Hkv, S, D, num_pages, page_size, max_pages;
   int64_t window;                            /* keys a query sees, itself among them; 0: all before it */
-  double scale, softcap;                     /* softcap 0: none */
+  double scale, softcap;                     /* from 1e-30 to 1e30; softcap 0: none */
   int32_t cache_type, index_flags;
 } kfmi_decode_args;
 

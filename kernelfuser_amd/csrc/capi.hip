@@ -571,8 +571,9 @@ int kfmi_attention_decode_bf16(const kfmi_decode_args *a, void *stream) {
   KFMI_TRY(check_index(a->lengths, a->index_flags, KFMI_I64_LENGTHS, "lengths"));
   KFMI_TRY(check_cache(a->k_cache, a->v_cache, a->k_scale, a->v_scale, a->cache_stride, a->scale_stride, a->num_pages,
                        a->page_size, a->cache_type));
-  if (!(a->scale > 0.0)) return fail(KFMI_EINVAL, "scale must be > 0");
-  if (!(a->softcap >= 0.0)) return fail(KFMI_EINVAL, "softcap must be >= 0");
+  if (!(a->scale >= 1e-30 && a->scale <= 1e30)) return fail(KFMI_EINVAL, "scale must be from 1e-30 to 1e30");
+  if (a->softcap != 0.0 && !(a->softcap >= 1e-30 && a->softcap <= 1e30))
+    return fail(KFMI_EINVAL, "softcap must be 0 or from 1e-30 to 1e30");
   if (a->window < 0) return fail(KFMI_EINVAL, "window must be >= 0 (got %lld)", (long long)a->window);
   KFMI_TRY(check_work(a->work, a->work_bytes));
   KFMI_TRY(check_device());

@@ -419,10 +419,24 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
 #pragma unroll
         for (int i = 0; i < 8; ++i) sc[i] = z[t][i / 4][i & 3] * (FP8 ? ks[i] : p.score_scale);
         if (p.cap > 0.f) {
-          // cap * tanh(x / cap) with tanh y = 1 - 2 / (e^2y + 1); the score is 2 y log2(e) here
+          // cap * tanh(x / cap) with tanh y = 1 - 2 / (e^2y + 1); the score is w = 2 y log2(e) here.
+          // That is good to 2^-22 of the cap: 2^-15 in a score capped at 128.  Under a
+          // larger cap a small y has the series y (1 - y^2 / 3 + 2 y^4 / 15), below 1/16 good
+          // to 2^-26 of itself (for every cap it made 16 sequences of 4096 keys, 32 rows a head,
+          // 47.7 us; without it they take 46).
+          if (p.cap > 128.0f * 1.4427f) {
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            sc[i] = fmaf(-2.0f * p.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(sc[i]) + 1.0f), p.cap);
+            for (int i = 0; i < 8; ++i) {
+              const float y = sc[i] * 0.34657359027997264f, y2 = y * y;
+              const float near = p.cap * y * fmaf(y2, fmaf(y2, 0.13333333333f, -0.33333333333f), 1.0f);
+              const float far = fmaf(-2.0f * p.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(sc[i]) + 1.0f), p.cap);
+              sc[i] = fabsf(sc[i]) < 0.18033688f ? near : far;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              sc[i] = fmaf(-2.0f * p.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(sc[i]) + 1.0f), p.cap);
+          }
         }
         if (edge) {
 #pragma unroll

@@ -4,8 +4,8 @@
 // One pass over a row x: each lane keeps a running maximum m with
 //   z = sum e^(x - m),  t = sum e^(x - m) (x - m)
 // (rescaled when m grows: t' = a (t + (m - m') z), z' = a z, a = e^(m - m')),
-// so that logp = x[id] - m - log z and the entropy is log z - t / z; all of
-// it in units of log 2, which is what v_exp_f32 takes.  The
+// so that logp = x[id] - m - log z and the entropy is log z - t / z, the exponents in
+// units of log 2, which is what v_exp_f32 takes.  The
 // alternatives are one sorted list per wave, entry i in lane i, of
 // (value, index) as one whole number; a tile of logits is looked through only
 // where its maximum exceeds the list's last entry, which a row of random logits
@@ -229,13 +229,19 @@ __device__ __forceinline__ float wave_sum(float x, int lane) {
   return x;
 }
 
-// Running maximum and sums of one lane, wave or workgroup, in units of log 2:
-// y = x log2(e), z = sum 2^(y - m), t = sum 2^(y - m) (y - m).
+// A maximum that overflows in units of log 2 (a row of the type's lowest values, say).
+__device__ __forceinline__ bool is_huge(float m) { return !(fabsf(m) <= 1e38f); }
+
+// Running maximum m and sums of one lane, wave or workgroup:
+// z = sum 2^d, t = sum 2^d d with d = fma(x, log2(e), -b), b = m log2(e) rounded,
+// one instruction per logit; where b would overflow, d = (x - m) log2(e).
 struct Sums {
   float m, z, t;
   __device__ __forceinline__ void move(float to) {  // to >= m; to -infinity only from -infinity
+#pragma clang fp contract(off)  // both products are rounded, as b is
     // finite, for the product with a = 0; NaN (m and `to` are +infinity) meets a z that is NaN
-    const float dm = m == -INFINITY ? 0.f : fmaxf(m - to, -1e4f);
+    const float by = is_huge(to) ? (m - to) * L2E : m * L2E - to * L2E;
+    const float dm = m == -INFINITY ? 0.f : fmaxf(by, -1e4f);
     const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(dm);
     t = a * fmaf(dm, z, t);
     z = a * z;
@@ -321,12 +327,13 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
       vm[u] = fmaxf(vm[u], x[u * VEC + VEC - 1]);
       top = fmaxf(top, vm[u]);
     }
-    if (top * L2E > s.m) s.move(top * L2E);
-    float b = s.m == -INFINITY ? 0.f : s.m;
+    if (top > s.m) s.move(top);
+    float b = s.m == -INFINITY ? 0.f : s.m * L2E;
     // 0 * -infinity is NaN: a wave that meets -infinity does the tile again and goes on with the exponents
     // held above -1000, which costs an instruction per logit.
-    const Sums kept = s;
-    if (!ruled_out) {
+    const bool huge = __any(is_huge(s.m) && s.m != -INFINITY);
+    if (!ruled_out && !huge) {
+      const Sums kept = s;
 #pragma unroll
       for (int i = 0; i < NE; ++i) {
         const float d = fmaf(x[i], L2E, -b), e = __builtin_amdgcn_exp2f(d);
@@ -339,11 +346,21 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
       // computed again, not kept: 64 registers
       asm volatile("" : "+v"(b));
     }
+    if (!huge) {
 #pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      const float d = fmaf(x[i], L2E, -b), e = __builtin_amdgcn_exp2f(d);
-      s.z += e;
-      s.t = fmaf(e, fmaxf(d, -1000.0f), s.t);
+      for (int i = 0; i < NE; ++i) {
+        const float d = fmaf(x[i], L2E, -b), e = __builtin_amdgcn_exp2f(d);
+        s.z += e;
+        s.t = fmaf(e, fmaxf(d, -1000.0f), s.t);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NE; ++i) {
+        const float d = is_huge(s.m) && s.m != -INFINITY ? (x[i] - s.m) * L2E : fmaf(x[i], L2E, -b);
+        const float e = __builtin_amdgcn_exp2f(d);
+        s.z += e;
+        s.t = fmaf(e, fmaxf(d, -1000.0f), s.t);
+      }
     }
   summed:
     if constexpr (TOP) {
@@ -463,7 +480,9 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
   const float nan = __uint_as_float(0x7fc00000u);
   const bool none = !(all.z > 0.f);  // NaN, +infinity or no logit above -infinity
   const float lz = log2f(all.z);
-  auto logp = [&](float x) { return (fmaf(x, L2E, -all.m) - lz) * LN2; };
+  // log2 of the sum relative to m itself: b's rounding goes back in
+  const float lm = is_huge(all.m) ? lz : lz - fmaf(all.m, L2E, -(all.m * L2E));
+  auto logp = [&](float x) { return x - all.m - lm * LN2; };
   if (lane == 0) {
     const int64_t id = load_index(p.ids, p.ids64, n0 * p.is[0] + n1 * p.is[1]);
     const bool in = id >= 0 && id < p.V;

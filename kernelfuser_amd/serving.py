@@ -385,14 +385,16 @@ def attention_decode(q, k_cache, v_cache, pages, lengths, k_scale=None, v_scale=
         window = 0
     elif int(window) < 1:
         raise ValueError("window must be >= 1")
+    else:
+        window = min(int(window), 1 << 40)
     if softcap is None:
         softcap = 0.0
-    elif not 0.0 < softcap < float("inf"):
-        raise ValueError("softcap must be positive and finite")
+    elif not 1e-30 <= softcap <= 1e30:
+        raise ValueError("softcap must be from 1e-30 to 1e30")
     if scale is None:
         scale = d ** -0.5
-    elif not 0.0 < scale < float("inf"):
-        raise ValueError("scale must be positive and finite")
+    elif not 1e-30 <= scale <= 1e30:
+        raise ValueError("scale must be from 1e-30 to 1e30")
     if b * hq * s * d >= 2 ** 31:
         raise ValueError("Tensors must have fewer than 2**31 elements")
     if out is not None and (out.shape != qshape or out.dtype is not _BF16 or not out.is_contiguous()):
@@ -413,7 +415,7 @@ def attention_decode(q, k_cache, v_cache, pages, lengths, k_scale=None, v_scale=
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), 0 if k_scale is None else k_scale.data_ptr(),
             0 if k_scale is None else v_scale.data_ptr(), pages.data_ptr(), lengths.data_ptr(), out.data_ptr(), wp,
             wb, *qs, cs[0], cs[1], cs[2], *es, pages_stride, lengths.stride(0), b, hq, hk, s, d, num_pages, page,
-            max_pages, int(window), scale, softcap, kind, flags)
+            max_pages, window, scale, softcap, kind, flags)
 
     _call(index, "kfmi_attention_decode_bf16", packed, space)
     return out

@@ -115,6 +115,23 @@ def test_decode_large_scores_and_scale(gpu):
     _check(x, _decode(y))
     _check(x, _decode(y, scale=0.01), scale=0.01)
     _check(x, _decode(y, softcap=20.0), softcap=20.0)
+    _check(x, _decode(y, softcap=3e4), softcap=3e4)  # hardly a cap: scores far below it keep their digits
+    _check(x, _decode(y, softcap=1e12), softcap=1e12)
+
+
+@pytest.mark.parametrize("b,geom,s,kind", [(70, (4, 2, 128), 1, "bf16"), (300, (2, 1, 128), 2, "e4m3"), (2, (64, 1, 128), 4, "bf16"),
+                                           (3, (48, 1, 256), 3, "e4m3")])
+def test_decode_many_sequences_and_many_rows(gpu, b, geom, s, kind):
+    """More sequences than lanes of a wave, and more query rows than a pass takes, split sequences among them."""
+    announce(f"decode b={b} {geom} S={s} {kind}")
+    g = torch.Generator().manual_seed(b)
+    lens = torch.randint(0, 60, (b,), generator=g).tolist()
+    lens[0], lens[-1], lens[b // 2] = 1500, 700, 0
+    x = _batch(lens, geom, 32, kind, 71, s)
+    got = _decode(_gpu(x, gpu))
+    some = sorted({0, 1, b // 2, b - 1, min(64, b - 1), min(65, b - 1)})
+    part = {"q": x["q"][some], "cache": x["cache"], "pages": x["pages"][some], "lengths": x["lengths"][some]}
+    _check(part, got[some])
 
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])

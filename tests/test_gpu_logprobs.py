@@ -93,6 +93,28 @@ def test_logprobs_rows_that_are_hard(gpu, kind):
     _compare(x, ids, top, [torch.stack([o[j] for o in one]) for j in range(4)])
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_logprobs_lowest_and_largest_values(gpu, kind):
+    """Masks of the type's lowest value, whole rows of it, and logits next to the type's largest."""
+    announce(f"logprobs lowest values {kind}")
+    v, top, t = 9001, 8, TYPES[kind]
+    low, big = torch.finfo(t).min, torch.finfo(t).max
+    g = torch.Generator().manual_seed(9)
+    rows = [torch.full((v,), low), torch.full((v,), big), torch.full((v,), low), torch.full((v,), low),
+            torch.randn(v, generator=g), torch.full((v,), -math.inf), torch.full((v,), low)]
+    rows[2][[4, 5000, 9000]] = torch.tensor([1.0, 2.0, 0.5])
+    rows[3][77] = low / 2
+    rows[4][100:200] = big
+    rows[4][300] = low
+    rows[5][8] = low
+    rows[6][::3] = -math.inf
+    x = torch.stack(rows).to(t)
+    ids = torch.tensor([5, 6, 5000, 77, 150, 8, 1])
+    _compare(x, ids, top, kf.token_logprobs(x.to(gpu), ids.to(gpu), top))
+    one = [kf.token_logprobs(x[i].to(gpu), ids[i].to(gpu), top) for i in range(len(rows))]
+    _compare(x, ids, top, [torch.stack([o[j] for o in one]) for j in range(4)])
+
+
 def test_logprobs_views(gpu):
     """Shifted logits of a batch, rows that do not start on 16 bytes, ids with strides, vectors and empty batches."""
     announce("logprobs views")
