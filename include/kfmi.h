@@ -306,7 +306,8 @@ int kfmi_launch_factored_attention_bf16(const void *q, const void *k, const void
  * Indices (positions, slots, pages, lengths, ids) are int32, or int64 where
  * the KFMI_I64_* flag says so.  They are on the device, so a wrong one is not an
  * error code: no entry point reads or writes out of range for any value,
- * and what a wrong one reaches is NaN, as each function says.
+ * and what a wrong one reaches is NaN, as each function says.  Nothing else may
+ * write them while a call that reads them runs.
  * ------------------------------------------------------------------------- */
 #define KFMI_CACHE_BF16 0
 #define KFMI_CACHE_E4M3 1
@@ -374,6 +375,8 @@ typedef struct {
  * is a cached row that no query sees; what those hold (NaN, infinities) does not matter.
  * A V row with a value that is not finite makes the outputs of the queries that see
  * it what the formula gives, or, where only some of the S queries see it, NaN throughout.
+ * Scores and the sums of weight (at most 1) times V are 32-bit floats, which
+ * values near the end of bf16's range can overflow.  out may be q where q is contiguous.
  * A length below 0 or above max_pages * page_size, or a page outside the cache among
  * those that a query sees, makes the sequence's outputs NaN.
  *
@@ -389,7 +392,7 @@ int kfmi_attention_decode_bf16(const kfmi_decode_args *args, void *stream);
 #define KFMI_DECODE_COUNTER_BYTES 8192
 
 /* Bytes of the workspace of kfmi_attention_decode_bf16 for these arguments (pointers and
- * strides are ignored) on the current device, into *bytes. */
+ * strides are ignored), into *bytes. */
 int kfmi_attention_decode_workspace(const kfmi_decode_args *args, int64_t *bytes);
 
 typedef struct {
@@ -444,7 +447,7 @@ int kfmi_token_logprobs(const kfmi_logprobs_args *args, void *stream);
 #define KFMI_LOGPROBS_COUNTER_BYTES 8192
 
 /* Bytes of the workspace of kfmi_token_logprobs for these arguments (pointers and strides are
- * ignored) on the current device, into *bytes. */
+ * ignored), into *bytes. */
 int kfmi_token_logprobs_workspace(const kfmi_logprobs_args *args, int64_t *bytes);
 
 #ifdef __cplusplus

@@ -797,7 +797,8 @@ hipError_t launch_decode(const kfmi_decode_args &a, hipStream_t stream) {
   p.pages64 = a.index_flags & KFMI_I64_PAGES;
   p.len64 = a.index_flags & KFMI_I64_LENGTHS;
   constexpr double log2e = 1.4426950408889634;
-  p.score_scale = (float)(a.softcap > 0 ? 2.0 * log2e * a.scale / a.softcap : a.scale * log2e);
+  // (a ratio beyond a float's range caps any score but 0)
+  p.score_scale = (float)(a.softcap > 0 ? fmin(2.0 * log2e * a.scale / a.softcap, 3.0e38) : a.scale * log2e);
   p.cap = (float)(a.softcap * log2e);
   const int64_t need = decode_workspace_bytes(a);
   if (need > 0 && a.work && a.work_bytes >= need) {

@@ -47,6 +47,8 @@ class Session:
         self.attentions = [m for m in model.modules() if type(m).__name__ == "Qwen3Attention"]
         if not self.attentions:
             raise RuntimeError("no Qwen3Attention modules found")
+        if any(getattr(m, "sliding_window", None) is not None for m in self.attentions):
+            raise ValueError("layers with a sliding window are not supported (the prefill has none)")
         dev = next(model.parameters()).device
         first = self.attentions[0]
         d, hkv = first.head_dim, first.k_proj.weight.shape[0] // first.head_dim
@@ -129,11 +131,12 @@ class Session:
     def capture(self):
         """Records the step in a HIP graph; later steps replay it.  The returned logits are then
         one tensor, overwritten by the next step."""
+        if self.filled >= self.max_length:
+            raise ValueError("the session's max_length is reached")
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):  # warm up outside the capture; what this writes, the next step writes again
             kept = self.lengths.clone()
-            self.lengths.clamp_(max=self.max_length - 1)
             self._step()
             self.lengths.copy_(kept)
         torch.cuda.current_stream().wait_stream(side)
@@ -152,7 +155,8 @@ class Session:
 def generate(model, ids, new_tokens: int, kind: str = "bf16", page_size: int = 64, graph: bool = False,
              session: Session | None = None):
     """Greedy continuation of the prompts ``ids`` [B,S]: a dict of ``tokens``,
-    ``logprobs`` and ``entropy`` [B,new_tokens] and ``prompt_logprobs`` [B,S-1]."""
+    ``logprobs`` and ``entropy`` [B,new_tokens] and ``prompt_logprobs`` [B,S-1].
+    Where the model's logits are no distribution (NaN) the token is -1, and the sequence goes on with token 0."""
     if new_tokens < 1:
         raise ValueError("new_tokens must be >= 1")
     s = session or Session(model, ids.shape[0], ids.shape[1] + new_tokens, kind, page_size)
@@ -165,7 +169,7 @@ def generate(model, ids, new_tokens: int, kind: str = "bf16", page_size: int = 6
         best = token_logprobs(last, ids[:, -1], 1)
         got.append((best.top_ids[:, 0], best.top_logprobs[:, 0], best.entropy))
         if i + 1 < new_tokens:
-            last = s.step(got[-1][0])
+            last = s.step(got[-1][0].clamp(min=0))
     tokens, logp, entropy = (torch.stack(t, dim=1) for t in zip(*got))
     return {"tokens": tokens, "logprobs": logp, "entropy": entropy, "prompt_logprobs": scored.logprobs}
 

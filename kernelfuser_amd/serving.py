@@ -18,7 +18,8 @@ of page ``z // page_size``.
 Indices (positions, slots, pages, lengths, ids) are int32 or int64 tensors on
 the device.  Their values are not checked on the host, which would have to wait
 for the GPU; the kernels never leave the tensors whatever the values are, and
-answer a wrong one with NaN, as each function says.
+answer a wrong one with NaN, as each function says.  Other work may not write them
+while a call that reads them runs.
 """
 from __future__ import annotations
 
@@ -223,7 +224,7 @@ def norm_rope_to_cache(q, k, v, gq, gk, cos, sin, positions, slots, k_cache, v_c
         raise ValueError("Pass both rotary tables (cos and sin) or neither")
     if k is None or v is None or gk is None or (q is not None and gq is None):
         raise ValueError("Expected k, v and gk (and gq with q)")
-    _check_grad("norm_rope_to_cache", q, k, v, gq, gk, cos, sin)
+    _check_grad("norm_rope_to_cache", q, k, v, gq, gk, cos, sin, k_cache, v_cache)
     shape, d1 = k.shape, (k.shape[-1],)
     if len(shape) != 4 or v.shape != shape:
         raise ValueError("Expected q [B,Hq,S,D] and k, v [B,Hkv,S,D]")
@@ -316,6 +317,7 @@ def cache_to_dense(k_cache, v_cache, pages, lengths, max_length, k_scale=None, v
     sequence's pages in order; ``lengths`` ``[B]``.  Rows behind a sequence's
     length are zeros.  Rows of a page outside the cache, and all rows of a sequence whose length is
     negative or more than its pages hold, are NaN."""
+    _check_grad("cache_to_dense", k_cache, v_cache)
     shape, cs, es, kind = _check_cache(k_cache, v_cache, k_scale, v_scale)
     num_pages, hk, page, d = shape
     b, l = lengths.shape[0] if lengths.ndim == 1 else 0, int(max_length)
@@ -348,7 +350,7 @@ def cache_to_dense(k_cache, v_cache, pages, lengths, max_length, k_scale=None, v
 def attention_decode(q, k_cache, v_cache, pages, lengths, k_scale=None, v_scale=None, *, scale=None, window=None,
                      softcap=None, out=None, work=None):
     """Attention of each sequence's last S tokens over its paged cache; returns
-    ``out`` ``[B,Hq,S,D]`` BF16.
+    ``out`` ``[B,Hq,S,D]`` BF16 (which may be a contiguous ``q``).
 
     ``q`` ``[B,Hq,S,D]``: prepared queries (``norm_rope_to_cache``'s ``qn``) of
     any strides, 1 <= S <= 16: one token per sequence, or a few drafted ones.  ``pages`` ``[B,max_pages]``: each
@@ -369,7 +371,7 @@ def attention_decode(q, k_cache, v_cache, pages, lengths, k_scale=None, v_scale=
     graph is captured, one of the graph's own, zeroed on each replay.  The
     result's bits depend on the lengths in the batch, not on timing.
     """
-    _check_grad("attention_decode", q)
+    _check_grad("attention_decode", q, k_cache, v_cache)
     qshape = q.shape
     if len(qshape) != 4 or q.dtype is not _BF16:
         raise ValueError("Expected q [B,Hq,S,D] in BF16")

@@ -66,12 +66,13 @@ def decode_bound(d, n, size, top, softcap):
     """Relative error of a softmax weight, times two for numerator and denominator.
 
     A score is a 32-bit sum of d exact products: at most (d + 3) roundings of 2^-24 of the sum of the products' sizes
-    (`size`, scaled); the cap adds a division, a tanh good to 2^-21 of the cap, or of the score where that is
-    below a sixteenth of the cap, and products.  exp adds 2^-22 for its
+    (`size`, scaled); the cap adds a division, a tanh good to 2^-21 of the cap (above 128 also to that of a score
+    below a sixteenth of the cap; 1 - 2 / (e^2y + 1) alone subtracts numbers near 1, so its error is the cap's), and products.  exp adds 2^-22 for its
     own error, and its argument, a difference of scores times log2(e), three roundings of at most 2 * top.  A weight is split into two bf16 numbers
     for the product with V, which keeps 2^-16 of it, and sums of n terms in 32 bits add at most (n + 16) 2^-24."""
     u = 2.0 ** -24
-    score = (d + 3) * u * size + (min(softcap, 16 * top) * 2.0 ** -21 + 6 * u * top if softcap else 0.0)
+    reach = min(softcap, 16 * top) if softcap and softcap > 128 else softcap
+    score = (d + 3) * u * size + (reach * 2.0 ** -21 + 6 * u * top if softcap else 0.0)
     return 2 * (score + 2.0 ** -22 + 8 * u * top) + 2.0 ** -16 + 2 * (n + 16) * u
 
 

@@ -287,3 +287,27 @@ def test_decode_own_workspace_is_left_ready(gpu):
     for _ in range(3):
         assert torch.equal(_decode(y, work=work), want)
         assert int(work[:8192].sum()) == 0
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_decode_shared_pages_and_in_place(gpu, kind):
+    """Sequences that share a prefix's pages, one sequence twice, one page several times in a row; out is q."""
+    announce(f"decode shared pages {kind}")
+    x = _batch([700, 700, 333, 64, 700], (32, 2, 128), 64, kind, seed=41, s=2)
+    x["pages"][1, :8] = x["pages"][0, :8]
+    x["pages"][4] = x["pages"][0]
+    x["q"][4] = x["q"][0]
+    x["pages"][2, :5] = 7
+    y = _gpu(x, gpu)
+    got = _decode(y)
+    _check(x, got)
+    assert _decode(y, out=y["q"]) is y["q"] and torch.equal(y["q"], got)
+
+
+def test_decode_ratio_of_scale_and_cap_beyond_32_bits(gpu):
+    """A cap of 1e-30 under a scale of 1e30: scores of at most 1e-30 whatever q . k is, 0 included, so every key has
+    the same weight to 1e-30, as under any other scale."""
+    announce("decode extreme scale over cap")
+    x = _batch([40], (2, 1, 128), 16, "bf16", seed=43)
+    x["q"][0, 1] = 0
+    _check(x, _decode(_gpu(x, gpu), scale=1e30, softcap=1e-30), softcap=1e-30)

@@ -128,3 +128,39 @@ def test_session_refusals(gpu, model):
         s.step(torch.zeros(1, dtype=torch.long, device=gpu))
     with pytest.raises(ValueError, match="new_tokens"):
         gen.generate(model, torch.zeros(1, 4, dtype=torch.long, device=gpu), 0)
+
+
+def test_full_session_is_not_captured_and_windows_are_refused(gpu, model):
+    """The warm-up of a capture writes the next token's rows, which a full session does not have."""
+    announce("capture of a full session")
+    s = gen.Session(model, 1, 4)
+    s.prefill(torch.arange(4, device=gpu)[None])
+    before = s.dense(0)
+    with pytest.raises(ValueError, match="max_length"):
+        s.capture()
+    assert all(torch.equal(a, b) for a, b in zip(before, s.dense(0)))
+    attention = s.attentions[0]
+    kept = attention.sliding_window
+    attention.sliding_window = 8
+    try:
+        with pytest.raises(ValueError, match="sliding window"):
+            gen.Session(model, 1, 4)
+    finally:
+        attention.sliding_window = kept
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_generation_goes_on_where_logits_are_nan(gpu, model, graph):
+    """Token -1 is no row of the embedding: the model is never given it."""
+    announce(f"generate with NaN logits graph={graph}")
+    norm = model.model.norm.weight
+    kept = norm.detach().clone()
+    with torch.no_grad():
+        norm.fill_(float("nan"))
+    try:
+        got = gen.generate(model, torch.arange(6, device=gpu).view(2, 3), 4, graph=graph)
+    finally:
+        with torch.no_grad():
+            norm.copy_(kept)
+    assert bool((got["tokens"] == -1).all())
+    assert all(bool(torch.isnan(got[k]).all()) for k in ("logprobs", "entropy", "prompt_logprobs"))

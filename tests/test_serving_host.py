@@ -310,3 +310,20 @@ def test_logprobs_reference():
 
 def test_packed_structures_are_bytes_for_one_call():
     assert isinstance(_dec(), bytes) and struct.calcsize("P") == 8
+
+
+def test_gradients_of_a_cache_are_refused():
+    """A cache that is a leaf (a learned prefix) would get no gradient: every op says so."""
+    args, kw = _append_args()
+    for i in (0, 1):
+        c = _cpu_cache()
+        c[i].requires_grad_()
+        with pytest.raises(ValueError, match="forward-only"):
+            kf.norm_rope_to_cache(*args[:9], *c, **kw)
+        pages, lengths = torch.zeros(2, 2, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+        with pytest.raises(ValueError, match="forward-only"):
+            kf.attention_decode(_z(2, 4, 1, 128), c[0], c[1], pages, lengths)
+        with pytest.raises(ValueError, match="forward-only"):
+            kf.cache_to_dense(c[0], c[1], pages, lengths, 8)
+        with torch.no_grad(), pytest.raises(ValueError, match="GPU device"):
+            kf.cache_to_dense(c[0], c[1], pages, lengths, 8)
