@@ -35,6 +35,7 @@ constexpr int WV = 4;            // waves per workgroup
 constexpr int NTHR = 64 * WV;
 constexpr int UNIT = 32 * WV;    // keys per unit of work
 constexpr int SC1 = 16;          // cache policy of agent-coherent accesses
+constexpr float LARGE_CAP = 128.0f * 1.44269504f;  // caps from here keep small scores' digits, see the kernel
 
 struct DecodeParams {
   const uint16_t *q;
@@ -50,8 +51,9 @@ struct DecodeParams {
   int capacity, window;
   int page_shift, page_mask;
   bool pages64, len64;
-  float score_scale;  // of q . k: to the exponent of 2 (cap 0), or to the argument 2 y log2(e) of the capped one
+  float score_scale;  // of q . k: to the argument 2 a log2(e) of c tanh a
   float cap;          // softcap * log2(e); 0: none
+  float slope, offset;  // of the scores (exponents of 2), see the kernel
 };
 
 // What a launch reads of one sequence.
@@ -135,13 +137,14 @@ __device__ __forceinline__ f32x4_t mfma(const u32x4_t &a, const u32x4_t &b, cons
                                                  0, 0);
 }
 
-__device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t w, bool high) {
-  return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, true)
-                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 1.0f, false));
+// Two e4m3 values of w times a scale, whose byte is the exponent of `scale`, as bf16: exact
+// for what a cache holds, NaN where the byte is 255.
+__device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t w, uint32_t scale, bool high) {
+  const float f = __uint_as_float(scale);
+  return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, f, true)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, f, false));
 }
-
-// The high bits of the bytes that are 255.
-__device__ __forceinline__ uint32_t ff_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & w & 0x80808080u; }
+__device__ __forceinline__ uint32_t scale_byte(uint32_t w, int i) { return ((w >> (8 * i)) & 255u) << 23; }
 
 // The d that element (m, t) of O^T is: lane group m of V's loads, product t.
 template <int D, bool FP8>
@@ -155,23 +158,27 @@ template <int D, bool FP8>
 struct VTile {
   static constexpr int W = FP8 ? D / 64 : D / 32;  // dwords per key and lane
   uint32_t w[8][W];
-  __device__ __forceinline__ u32x4_t operand(int t) const {
-    u32x4_t r;
+  uint32_t scale[FP8 ? 8 : 1];
+  // Values 2 x and 2 x + 1 of key j in bf16.
+  __device__ __forceinline__ uint32_t pair(int j, int x) const {
+    if constexpr (FP8) return bf16_of_e4m3(w[j][x / 2], scale[j], x & 1);
+    else return w[j][x];
+  }
+  // The operands of products 2 x and 2 x + 1.
+  __device__ __forceinline__ void operands(int x, u32x4_t (&a)[2]) const {
+    uint32_t c[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) c[j] = pair(j, x);
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
-      if constexpr (FP8) {
-        const uint32_t a = w[2 * y][t / 4], b = w[2 * y + 1][t / 4];
-        const uint32_t pair = __builtin_amdgcn_perm(b, a, t & 2 ? 0x07030602u : 0x05010400u);
-        r[y] = bf16_of_e4m3(pair, t & 1);
-      } else {
-        r[y] = __builtin_amdgcn_perm(w[2 * y + 1][t / 2], w[2 * y][t / 2], t & 1 ? 0x07060302u : 0x05040100u);
-      }
+      a[0][y] = __builtin_amdgcn_perm(c[2 * y + 1], c[2 * y], 0x05040100u);
+      a[1][y] = __builtin_amdgcn_perm(c[2 * y + 1], c[2 * y], 0x07060302u);
     }
-    return r;
   }
   // Whether a value of key j is an infinity or NaN.
   __device__ __forceinline__ bool odd(int j) const {
     bool any = false;
+    if constexpr (FP8) any = scale[j] == 255u << 23;
 #pragma unroll
     for (int x = 0; x < W; ++x) {
       const uint32_t u = w[j][x];
@@ -191,8 +198,9 @@ struct VTile {
 // arithmetic per byte and is faster with two waves where the registers allow them.
 constexpr int waves_per_simd(int d, bool fp8, int nt) { return fp8 && d * nt <= 256 ? 2 : 1; }
 
-// MULTI: S > 1.
-template <int D, bool FP8, int NT, bool MULTI>
+// GENERAL: several queries or a cap.  Without it (one token per sequence, no cap) neither is in the code: one sequence
+// of 333 keys 8.2 instead of 8.7 us, 64 of up to 8192 in bf16 175 instead of 176.5.
+template <int D, bool FP8, int NT, bool GENERAL>
 __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kernel(DecodeParams p) {
   constexpr int NK = D / 32;    // matrix steps of q . k
   constexpr int ND = D / 16;    // products of P V
@@ -209,6 +217,7 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
   __shared__ uint32_t arrived;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, c = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const float offset = GENERAL ? p.offset : 0.f;
   const uint32_t ipb = (uint32_t)(p.hk * p.rblocks);  // items (head, block of rows) per sequence
 
   // This workgroup's share [g0, g1) of all units, the sequences in the order
@@ -296,7 +305,7 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
 #pragma unroll
       for (int k = 0; k < (FP8 ? NK / 2 : NK); ++k)
         kw[t][k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t *>(kb[t] + (n * row + 16 * c + 64 * k)));
-      if constexpr (FP8) ksw[t] = *reinterpret_cast<const uint32_t *>(ksb[t] + 4 * c);
+      if constexpr (FP8) ksw[t] = ksb[t][n];
     }
   };
   auto load_v = [&]() {
@@ -380,33 +389,14 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
         for (int k = 0; k < NK; ++k) {
           u32x4_t a;
           if constexpr (FP8) {
-            const uint32_t x0 = kw[u][k / 2][2 * (k & 1)], x1 = kw[u][k / 2][2 * (k & 1) + 1];
-            a = u32x4_t{bf16_of_e4m3(x0, false), bf16_of_e4m3(x0, true), bf16_of_e4m3(x1, false), bf16_of_e4m3(x1, true)};
+            const uint32_t x0 = kw[u][k / 2][2 * (k & 1)], x1 = kw[u][k / 2][2 * (k & 1) + 1], ks = ksw[u] << 23;
+            a = u32x4_t{bf16_of_e4m3(x0, ks, false), bf16_of_e4m3(x0, ks, true), bf16_of_e4m3(x1, ks, false),
+                        bf16_of_e4m3(x1, ks, true)};
           } else {
             a = kw[u][k];
           }
 #pragma unroll
           for (int t = 0; t < NT; ++t) z[t][u] = mfma(a, qf[t][k], z[t][u]);
-        }
-      }
-      float ks[FP8 ? 8 : 1], vs[FP8 ? 8 : 1];
-      if constexpr (FP8) {
-        const uint32_t odd = ff_bytes(ksw[0]) | ff_bytes(ksw[1]) | ff_bytes(vsw[0]) | ff_bytes(vsw[1]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int sh = 8 * (i & 3);
-          ks[i] = __builtin_amdgcn_ldexpf(p.score_scale, (int)((ksw[i / 4] >> sh) & 255u) - 127);
-          vs[i] = __builtin_amdgcn_ldexpf(1.0f, (int)((vsw[i / 4] >> sh) & 255u) - 127);
-        }
-        if (edge || __any(odd != 0)) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int sh = 8 * (i & 3);
-            if (((ksw[i / 4] >> sh) & 255u) == 255u) ks[i] = __uint_as_float(0x7fc00000u);
-            if (((vsw[i / 4] >> sh) & 255u) == 255u) vs[i] = __uint_as_float(0x7fc00000u);
-            const int j = j0 + 16 * (i / 4) + 4 * c + (i & 3);
-            if (j < s.lo || j >= s.len) ks[i] = vs[i] = 0.f;  // one that is not seen may be NaN
-          }
         }
       }
       __builtin_amdgcn_sched_barrier(0);  // the loads take the registers of what they follow
@@ -415,40 +405,39 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
       u32x4_t ph[NT], pl[NT];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        float sc[8];
+        // Scores are p.slope * y + p.offset: y is q . k, or under a cap c with
+        // c tanh a = c - 2 c / (e^2a + 1) that last quotient's -1 / (e^2a + 1).  The sum is good to 2^-22 of the
+        // cap: 2^-15 in a score capped at 128.  Under a larger cap y is the score, where a
+        // is small by the series a (1 - a^2 / 3 + 2 a^4 / 15), below 1/16 good
+        // to 2^-26 of itself (for every cap it made 16 sequences of 4096 keys, 32 rows a head,
+        // 47.7 us; without it they take 46).
+        float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sc[i] = z[t][i / 4][i & 3] * (FP8 ? ks[i] : p.score_scale);
-        if (p.cap > 0.f) {
-          // cap * tanh(x / cap) with tanh y = 1 - 2 / (e^2y + 1); the score is w = 2 y log2(e) here.
-          // That is good to 2^-22 of the cap: 2^-15 in a score capped at 128.  Under a
-          // larger cap a small y has the series y (1 - y^2 / 3 + 2 y^4 / 15), below 1/16 good
-          // to 2^-26 of itself (for every cap it made 16 sequences of 4096 keys, 32 rows a head,
-          // 47.7 us; without it they take 46).
-          if (p.cap > 128.0f * 1.4427f) {
+        for (int i = 0; i < 8; ++i) y[i] = z[t][i / 4][i & 3];
+        if (GENERAL && p.cap > 0.f) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            y[i] = -__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(y[i] * p.score_scale) + 1.0f);
+          if (p.cap > LARGE_CAP) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const float y = sc[i] * 0.34657359027997264f, y2 = y * y;
-              const float near = p.cap * y * fmaf(y2, fmaf(y2, 0.13333333333f, -0.33333333333f), 1.0f);
-              const float far = fmaf(-2.0f * p.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(sc[i]) + 1.0f), p.cap);
-              sc[i] = fabsf(sc[i]) < 0.18033688f ? near : far;
+              const float w = z[t][i / 4][i & 3] * p.score_scale, a = w * 0.34657359027997264f, a2 = a * a;
+              const float near = p.cap * a * fmaf(a2, fmaf(a2, 0.13333333333f, -0.33333333333f), 1.0f);
+              y[i] = fabsf(w) < 0.18033688f ? near : fmaf(2.0f * p.cap, y[i], p.cap);
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              sc[i] = fmaf(-2.0f * p.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(sc[i]) + 1.0f), p.cap);
           }
         }
         if (edge) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const int j = j0 + 16 * (i / 4) + 4 * c + (i & 3);
-            if (j < lo[t] || j >= hi[t]) sc[i] = -INFINITY;
+            if (j < lo[t] || j >= hi[t]) y[i] = -INFINITY;
           }
         }
-        float mx = sc[0];
+        float mx = y[0];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, sc[i]);
-        mx = fmaxf(max_rows4(mx), m[t]);
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, y[i]);
+        mx = fmaxf(fmaf(p.slope, max_rows4(mx), offset), m[t]);
         const float base = mx == -INFINITY ? 0.f : mx;  // no key so far: the weights below are 0
         if (__any(mx > m[t])) {
           const float alpha = __builtin_amdgcn_exp2f(m[t] - base);
@@ -461,23 +450,17 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
         float pr[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          pr[i] = __builtin_amdgcn_exp2f(sc[i] - base);
+          pr[i] = __builtin_amdgcn_exp2f(fmaf(p.slope, y[i], offset - base));
           sum += pr[i];
-          if constexpr (FP8) pr[i] *= vs[i];
-        }
-        if (FP8 && MULTI && edge) {  // a scale that this query does not see may be NaN
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (sc[i] == -INFINITY) pr[i] = 0.f;
         }
         l[t] += sum;
-        // p = hi + lo, both bf16 and both positive where p is: lo keeps 2^-7
+        // p = hi + lo, both bf16.  For a bf16 cache both are positive where p is: lo keeps 2^-7
         // to 2^-6 of p, so that an infinite v, which meets both, stays an infinity.
         float lo_[8];
         uint32_t hb[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          hb[i] = __float_as_uint(pr[i] * 0.9921875f);
+          hb[i] = __float_as_uint(FP8 ? pr[i] : pr[i] * 0.9921875f);
           lo_[i] = pr[i] - __uint_as_float(hb[i] & 0xffff0000u);
         }
 #pragma unroll
@@ -487,12 +470,16 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
         }
       }
 
+      if constexpr (FP8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v.scale[j] = scale_byte(vsw[j / 4], j & 3);
+      }
       if (edge) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int key = j0 + 16 * (j / 4) + 4 * c + (j & 3);
           bool drop = key < s.lo || key >= s.len;
-          if constexpr (MULTI) {
+          if constexpr (GENERAL) {
             // A value that is not finite, of a key that only some of the queries
             // see, would reach the others as 0 * NaN: the key is taken out, and the
             // rows that see it are NaN.
@@ -507,14 +494,18 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
           if (drop) {
 #pragma unroll
             for (int x = 0; x < VTile<D, FP8>::W; ++x) v.w[j][x] = 0u;
+            if constexpr (FP8) v.scale[j] = 0u;
           }
         }
       }
 #pragma unroll
-      for (int d = 0; d < ND; ++d) {
-        const u32x4_t a = v.operand(d);
+      for (int d = 0; d < ND; d += 2) {
+        u32x4_t a[2];
+        v.operands(d / 2, a);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) acc[t][d] = mfma(a, pl[t], mfma(a, ph[t], acc[t][d]));
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) acc[t][d + x] = mfma(a[x], pl[t], mfma(a[x], ph[t], acc[t][d + x]));
       }
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (more.value) load_v();
@@ -738,22 +729,22 @@ Plan plan_of(const kfmi_decode_args &a) {
   return r;
 }
 
-template <int D, bool FP8, int NT, bool MULTI>
+template <int D, bool FP8, int NT, bool GENERAL>
 hipError_t launch_decode_t(const DecodeParams &p, int64_t grid, hipStream_t stream) {
-  hipLaunchKernelGGL((decode_kernel<D, FP8, NT, MULTI>), dim3((unsigned)grid), dim3(NTHR), 0, stream, p);
+  hipLaunchKernelGGL((decode_kernel<D, FP8, NT, GENERAL>), dim3((unsigned)grid), dim3(NTHR), 0, stream, p);
   static const std::string name = [] {
     char b[96];
-    snprintf(b, sizeof(b), "decode_kernel<%d, %s, %d, %s>", D, tf(FP8), NT, tf(MULTI));
+    snprintf(b, sizeof(b), "decode_kernel<%d, %s, %d, %s>", D, tf(FP8), NT, tf(GENERAL));
     return std::string(b);
   }();
-  launch_log_add(reinterpret_cast<const void *>(&decode_kernel<D, FP8, NT, MULTI>), name.c_str(), grid, NTHR);
+  launch_log_add(reinterpret_cast<const void *>(&decode_kernel<D, FP8, NT, GENERAL>), name.c_str(), grid, NTHR);
   launch_log_plan("split=%d rblocks=%d", p.counters != nullptr, p.rblocks);
   return hipGetLastError();
 }
 
 template <int D, bool FP8, int NT>
 hipError_t launch_decode_s(const DecodeParams &p, int64_t grid, hipStream_t stream) {
-  return p.S > 1 ? launch_decode_t<D, FP8, NT, true>(p, grid, stream) : launch_decode_t<D, FP8, NT, false>(p, grid, stream);
+  return p.S > 1 || p.cap > 0.f ? launch_decode_t<D, FP8, NT, true>(p, grid, stream) : launch_decode_t<D, FP8, NT, false>(p, grid, stream);
 }
 
 template <int D, bool FP8>
@@ -797,9 +788,11 @@ hipError_t launch_decode(const kfmi_decode_args &a, hipStream_t stream) {
   p.pages64 = a.index_flags & KFMI_I64_PAGES;
   p.len64 = a.index_flags & KFMI_I64_LENGTHS;
   constexpr double log2e = 1.4426950408889634;
-  // (a ratio beyond a float's range caps any score but 0)
-  p.score_scale = (float)(a.softcap > 0 ? fmin(2.0 * log2e * a.scale / a.softcap, 3.0e38) : a.scale * log2e);
   p.cap = (float)(a.softcap * log2e);
+  // (a ratio of scale and cap beyond a float's range caps any score but 0)
+  p.score_scale = a.softcap > 0 ? (float)fmin(2.0 * log2e * a.scale / a.softcap, 3.0e38) : 0.0f;
+  p.slope = a.softcap == 0 ? (float)(a.scale * log2e) : p.cap > LARGE_CAP ? 1.0f : 2.0f * p.cap;
+  p.offset = a.softcap == 0 || p.cap > LARGE_CAP ? 0.0f : p.cap;
   const int64_t need = decode_workspace_bytes(a);
   if (need > 0 && a.work && a.work_bytes >= need) {
     p.counters = (int *)a.work;
