@@ -176,6 +176,7 @@ struct TopList {
   }
   // Another list.
   __device__ __forceinline__ void merge(uint64_t x, int lane, int top) {
+    if (lane_of(x, 0) <= tau) return;
     merge_up(exchange<32>(exchange<16>(exchange<15>(x, lane), lane), lane), lane, top);
   }
   // One key per lane (0: none): a few are put in one by one, some 250 cycles each,
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
   constexpr int SIZE = 16 / VEC;
   constexpr int NE = LU * VEC;  // logits of a lane and tile
   __shared__ uint64_t keys[4][TOPM];
-  __shared__ uint64_t found[TOP ? 4 : 1][TOP ? 64 + 64 * VEC : 1];
+  __shared__ uint64_t found[TOP ? 4 : 1][TOP ? 128 : 1];
   __shared__ float sums[4][3];
   __shared__ uint32_t arrived;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -290,6 +291,16 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
     for (int u = 0; u < LU; ++u)
       raw[u] = __builtin_nontemporal_load(
           reinterpret_cast<const u32x4_t *>(first - head * SIZE + (int64_t)(vt + 64 * u + lane) * 16));
+  };
+  // What may belong to the list: values above the bar, gathered in LDS until there are more than 64.
+  float bar = -INFINITY, seen = -INFINITY;
+  int have = 0, tiles = 0, rank_at = 1;
+  auto flush = [&] {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int o = 0; o < have; o += 64) list.insert(o + lane < have ? found[w][o + lane] : 0ull, lane, p.top);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    have = 0;
+    bar = fmaxf(bar, key_value(list.tau));
   };
   const int vt0 = v0 + (alone ? 0 : w) * (64 * LU), stride = p.waves * 64 * LU;
   bool requested = vt0 < v1 && inner(vt0);
@@ -365,38 +376,50 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
   summed:
     if constexpr (TOP) {
       const uint32_t i0 = (uint32_t)((vt + lane) * VEC - head);  // index of x[0]
-      if (__any(top > key_value(list.tau))) {
-        // What may belong is gathered in LDS and enters the list 64 at a time.  In
-        // the first tile that is what reaches the top-th largest of the lanes' maxima,
-        // later what exceeds the list's last entry (an equal one has a higher index).
-        const bool begin = list.tau == 0;
-        const float tv = key_value(begin ? nth_largest(value_key(top), lane, p.top) : (uint32_t)(list.tau >> 32));
-        auto belongs = [&](float y) { return (y > tv || (begin && y == tv)) && y > -INFINITY; };
-        int have = 0;
-        auto flush = [&] {
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          for (int o = 0; o < have; o += 64) list.insert(o + lane < have ? found[w][o + lane] : 0ull, lane, p.top);
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          have = 0;
-        };
-#pragma unroll
-        for (int u = 0; u < LU; ++u) {
-          if (!__any(belongs(vm[u]))) continue;
-          if (have > 64) flush();
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float y = x[u * VEC + e];
-            const bool in = belongs(y);
-            const uint64_t ins = __ballot(in);
-            if (ins) {
-              if (in) found[w][have + __builtin_popcountll(ins & ((1ull << lane) - 1))] = rank_key(y, i0 + (uint32_t)(u * 64 * VEC + e));
-              have += __builtin_popcountll(ins);
-            }
+      ++tiles;
+      seen = fmaxf(seen, top);
+      if (__any(top > bar)) {
+        // The lanes' maxima of all tiles so far bound the top-th largest from below; they are
+        // ranked again whenever the number of tiles has doubled.  What exceeds the bar is gathered in LDS and enters
+        // the list 64 at a time.  A value equal to a bar that was there before this tile has `top`
+        // others of lower indices before it; one equal to a bar that this tile raises may not.
+        float above = bar;
+        if (tiles >= rank_at) {
+          const uint32_t to = nth_largest(value_key(seen), lane, p.top);
+          rank_at = 2 * tiles;
+          if (key_value(to) > bar) {
+            bar = key_value(to);
+            above = key_value(to - (to == 0x80000000u ? 2 : 1));  // the next lower number
           }
         }
-        flush();
+        uint32_t mine = 0;  // this lane's
+#pragma unroll
+        for (int e = NE - 1; e >= 0; --e) mine = mine << 1 | (x[e] > above ? 1u : 0u);
+        for (;;) {  // one of each lane
+          const uint64_t who = __ballot(mine != 0);
+          if (!who) break;
+          if (have > 64) flush();
+          const int e = mine ? __builtin_ctz(mine) : 0;
+          uint32_t y[NE];  // x[e], bit by bit of e
+#pragma unroll
+          for (int k = 0; k < NE; ++k) y[k] = __float_as_uint(x[k]);
+#pragma unroll
+          for (int o = 1; o < NE; o *= 2) {
+            const uint32_t m = e & o ? ~0u : 0u;
+#pragma unroll
+            for (int k = 0; k < NE; k += 2 * o) y[k] = (y[k + o] & m) | (y[k] & ~m);
+          }
+          if (mine)
+            found[w][have + __builtin_popcountll(who & ((1ull << lane) - 1))] =
+                rank_key(__uint_as_float(y[0]), i0 + (uint32_t)(e / VEC * (64 * VEC) + e % VEC));
+          have += __builtin_popcountll(who);
+          mine &= mine - 1;
+        }
       }
     }
+  }
+  if constexpr (TOP) {
+    if (have > 0) flush();
   }
 
   // The lanes' sums and lists of all waves, in the first wave (lists: each wave's in LDS).
