@@ -177,6 +177,11 @@ struct TopList {
   // Another list.
   __device__ __forceinline__ void merge(uint64_t x, int lane, int top) {
     if (lane_of(x, 0) <= tau) return;
+    if (lane_of(key, 0) == 0) {
+      key = x;
+      tau = lane_of(x, top - 1);
+      return;
+    }
     merge_up(exchange<32>(exchange<16>(exchange<15>(x, lane), lane), lane), lane, top);
   }
   // One key per lane (0: none): a few are put in one by one, some 250 cycles each,
@@ -260,7 +265,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
   constexpr int VEC = vec_of<TYPE>();
   constexpr int SIZE = 16 / VEC;
   constexpr int NE = LU * VEC;  // logits of a lane and tile
-  __shared__ uint64_t keys[4][TOPM];
+  __shared__ uint64_t keys[4][TOPM], joined[TOPM];
   __shared__ uint64_t found[TOP ? 4 : 1][TOP ? 128 : 1];
   __shared__ float sums[4][3];
   __shared__ uint32_t arrived;
@@ -432,6 +437,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
       sums[w][2] = x.t;
     }
     if (TOP && lane < p.top) keys[w][lane] = list.key;
+    if (TOP && tid < TOPM) joined[tid] = 0ull;
     __syncthreads();
     if (w == 0) {
       const float top = fmaxf(fmaxf(sums[0][0], sums[1][0]), fmaxf(sums[2][0], sums[3][0]));
@@ -447,12 +453,23 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
     }
     return x;
   };
-  // The waves' lists as one, in the first wave.
+  // The waves' lists as one, in the first wave: a key's place is the number of larger ones in
+  // all four sorted lists, found by halving.
   auto join_lists = [&] {
-    if (TOP && w == 0 && !alone) {
+    if (!TOP || alone) return;
+    const uint32_t top = (uint32_t)p.top;
+    uint32_t larger[3] = {0, 0, 0};
+    for (uint32_t o = 1u << (31 - __builtin_clz(top)); o > 0; o /= 2) {
 #pragma unroll
-      for (int i = 1; i < 4; ++i) list.merge(lane < p.top ? keys[i][lane] : 0ull, lane, p.top);
+      for (int i = 0; i < 3; ++i) {
+        const uint32_t at = larger[i] + o;
+        larger[i] = (keys[(w + i + 1) & 3][min(at, top) - 1] > list.key) & (at <= top) ? at : larger[i];
+      }
     }
+    const uint32_t place = (uint32_t)lane + larger[0] + larger[1] + larger[2];
+    if (list.key != 0 && place < top) joined[place] = list.key;
+    __syncthreads();
+    if (w == 0) list.key = lane < p.top ? joined[lane] : 0ull;
   };
 
   Sums all = join_waves(s);
@@ -498,6 +515,7 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
     all = join_waves(s);
   }
 
+  join_lists();
   if (w != 0 && !alone) return;
   constexpr float LN2 = 0.693147180559945309417f;
   const float nan = __uint_as_float(0x7fc00000u);
@@ -513,7 +531,6 @@ __global__ __launch_bounds__(256) void logprobs_kernel(LogprobsParams p) {
     p.entropy[row] = none ? nan : (lz - all.t / all.z) * LN2;
   }
   if constexpr (TOP) {
-    join_lists();
     const int64_t out = (int64_t)row * p.top;
     if (none) {
       if (lane < p.top) {
