@@ -77,17 +77,20 @@ __device__ __forceinline__ Sequence sequence(const DecodeParams &p, int b) {
 }
 
 // Units of work per workgroup: an even share, but
-//  * where two workgroups per CU would have up to four units each, one has
-//    them all (e4m3, 32 sequences of 1024 keys: 19.2 instead of 21.2 us at D = 128, 29.0
-//    instead of 32.0 at D = 256; from eight units on two are faster, 31.7 instead of 32.7);
+//  * where two workgroups per CU would have up to four units each (eight at D = 256), one
+//    has them all (e4m3, 32 sequences of 1024 keys at D = 128: 17.4 instead of 20.6 us, 32 of 2048 at
+//    D = 256 49 instead of 54; with more two are faster, 64 of 1024 at D = 128 28.3 instead of 31.2,
+//    64 of up to 8192 at D = 256 180 instead of 189);
 //  * a sequence (`most` units, the longest) of up to three units is not split: the join
-//    takes as long as two (one of 333 keys: 9.2 instead of 9.7 us), and a longer
+//    takes as long as two (one of 333 keys: 9.3 instead of 9.5 us), and a longer
 //    one not into more parts than its join, some 2.5 us for 64 rows of
 //    parts, leaves worth it: units / parts * 1.2 us + rows * parts / 64 * 2.5 us is least at
-//    parts = sqrt(31 * units / rows) (8192 keys, 32 rows: 66 us in 32 parts).
-__device__ __forceinline__ uint32_t units_per_workgroup(uint32_t total, uint32_t most, uint32_t grid, uint32_t rows) {
+//    parts = sqrt(31 * units / rows) (one of 8192 keys, 32 rows a head: 33 us, 43 in as many parts as
+//    there are units; 64 rows 69 and 84).
+__device__ __forceinline__ uint32_t units_per_workgroup(uint32_t total, uint32_t most, uint32_t grid, uint32_t rows,
+                                                        uint32_t few) {
   uint32_t even = (total + grid - 1) / grid;
-  if (grid > 256 && even <= 4) even = (total + 255) / 256;
+  if (grid > 256 && even <= few) even = (total + 255) / 256;
   const uint32_t least = most <= 3 ? most : min(most, (uint32_t)__builtin_sqrtf((float)(most * rows) * (1.0f / 31.0f)));
   return max(even, max(least, 1u));
 }
@@ -195,7 +198,8 @@ struct VTile {
 
 // Waves per SIMD.  A wave alone on its SIMD reads bf16 as fast as two do, and half
 // the workgroups make half the parts of a split sequence; e4m3 takes twice the
-// arithmetic per byte and is faster with two waves where the registers allow them.
+// arithmetic per byte and is faster with two waves where the registers allow them (64
+// sequences of 4096 keys at D = 128: 92 instead of 104 us).
 constexpr int waves_per_simd(int d, bool fp8, int nt) { return fp8 && d * nt <= 256 ? 2 : 1; }
 
 // GENERAL: several queries or a cap.  Without it (one token per sequence, no cap) neither is in the code: one sequence
@@ -243,7 +247,7 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
   }
   most = (uint32_t)__builtin_amdgcn_readfirstlane((int)most);
   const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
-  const uint32_t per = units_per_workgroup(total, most, gridDim.x, (uint32_t)min(ROWS, p.rows));
+  const uint32_t per = units_per_workgroup(total, most, gridDim.x, (uint32_t)min(ROWS, p.rows), D / 32);
   const uint32_t g0 = blockIdx.x * per, g1 = min(g0 + per, total);
   if (g0 >= total) return;  // workgroup-uniform
   int b = __builtin_ctzll(__ballot(incl > g0));
@@ -409,8 +413,8 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
         // c tanh a = c - 2 c / (e^2a + 1) that last quotient's -1 / (e^2a + 1).  The sum is good to 2^-22 of the
         // cap: 2^-15 in a score capped at 128.  Under a larger cap y is the score, where a
         // is small by the series a (1 - a^2 / 3 + 2 a^4 / 15), below 1/16 good
-        // to 2^-26 of itself (for every cap it made 16 sequences of 4096 keys, 32 rows a head,
-        // 47.7 us; without it they take 46).
+        // to 2^-26 of itself (for every cap it would make 16 sequences of 4096 keys, 32 rows a head,
+        // 48 us; without it they take 45).
         float y[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = z[t][i / 4][i & 3];
