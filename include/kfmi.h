@@ -1,5 +1,7 @@
 /*
- * kfmi.h -- C ABI of the MI355X (gfx950) RoPE-aware attention prologue.
+ * kfmi.h -- C ABI of the MI355X (gfx950) RoPE-aware attention prologue, and of
+ * the serving ops that follow it (last section, with conventions of its own for
+ * strides and indices).
  *
  * The drop-in boundary for KernelFuser's attention-prologue path
  * (WenbinWang12/KernelFuser).  The reference has no native boundary: its

@@ -3,6 +3,12 @@
 //
 // Both are memory-bound: a row of D values is D/8 lanes of 8 values each (one
 // 16-lane DPP row at D = 128), 16 bytes of bf16 or 8 bytes of e4m3 per lane.
+//
+// Writing: norm y = bf16 chain of x / sqrt(mean x^2 + eps) * gamma, rotation y cos + partner sin at the
+// token's own table row (rows_common.h), then, for e4m3, y / 2^e rounded.  8192 tokens of 32 + 2 x 8 heads of
+// D = 128 take 35 us (205 MB, 5.9 TB/s), 4000 e4m3 tokens of 16 + 2 x 8 of D = 256 26 us (116 MB), where the
+// row arithmetic and the conversion fill 70% of the vector slots; one token 2.6 us, a launch.
+// Reading: 8 sequences of 4096 e4m3 keys, 8 heads of D = 256, 60 us (344 MB, 5.7 TB/s).
 #include <cstdio>
 #include <string>
 
@@ -29,7 +35,8 @@ struct WriteParams {
   float eps;
 };
 
-// Rows from which a lane takes four heads of its token instead of one.
+// Rows from which a lane takes four heads of its token instead of one (32 + 2 x 8 heads of D = 128:
+// 24576 rows 4.9 us with one, 5.6 with four; 98304 rows 14.9 and 10.9).
 constexpr int64_t WIDE_ROWS = 1 << 15;
 
 // Bytes (read and written) from which reading the cache back leaves the caches alone: what

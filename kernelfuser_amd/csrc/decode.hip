@@ -3,8 +3,10 @@
 //
 // out_i = sum_j softmax_j(cap(q_i . k_j * scale)) v_j over the keys that
 // query i sees.  Every key and value is read once per KV head, so the cache's bytes
-// bound the call: 4 * D * 2 bytes (bf16) per key and head against 4 * D * R flops for the R = group * S query rows
-// that share them, at most 64 rows a pass.  The design:
+// bound the call: 4 * D bytes (bf16) per key and head against 4 * D * R flops for the R = group * S query rows
+// that share them, at most 64 rows a pass (32 at D = 256).  64 sequences of 4096 keys, 8 heads of D = 128, take
+// 169 us (1.07 GB, 6.4 TB/s; a bare read of such pages reaches 6.8), one of 32768 28.4 us, one of 333 8.2; at 32
+// rows in e4m3 the softmax and the conversions bound it instead: 16 sequences of 4096 keys 41 us (137 MB).  The design:
 //
 //  * the R rows of a KV head are the columns of 16x16x32 matrix
 //    instructions: S^T = K Q^T with 16 keys, O^T = V^T P^T with 16 values of d.
@@ -16,7 +18,7 @@
 //    32 keys.  Nothing goes through LDS in the loop, no wave waits for another;
 //  * a weight is the sum of two bf16 numbers, two products each: its rounding to one
 //    would be as large as the result's own (2^-9), and the matrix
-//    units have time for it;
+//    units have time for it.  An e4m3 row becomes bf16, times its scale, in the conversion, exactly;
 //  * the work of a launch (units of 32 keys per wave, all heads and sequences)
 //    is dealt evenly to one round of workgroups, whatever the lengths: each
 //    finds its share by a scan of the lengths.  A head's sequence that

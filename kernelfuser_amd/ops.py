@@ -328,7 +328,7 @@ def optimized_attention(q, k, v, gq, gk, cos=None, sin=None, *, causal=False, mo
     and K, then runs the same attention.  ``norm_style``: ``'hf'`` rounds at HF's
     BF16 op boundaries, ``'legacy'`` casts x*inv*gamma once, ``'fp32'`` keeps the
     whole prologue in FP32 with one final rounding.  Forward only; projections,
-    KV caches and backward are out of scope.  Every argument error raises
+    KV caches are the serving ops' (``serving``), backward is out of scope.  Every argument error raises
     ``ValueError`` before anything is launched (rope:695-719).
     """
     if mode not in ("query", "unfused") or bn not in (64, 128):
