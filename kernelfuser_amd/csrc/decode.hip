@@ -82,7 +82,9 @@ __device__ __forceinline__ Sequence sequence(const DecodeParams &p, int b) {
 //  * where two workgroups per CU would have up to four units each (eight at D = 256), one
 //    has them all (e4m3, 32 sequences of 1024 keys at D = 128: 17.4 instead of 20.6 us, 32 of 2048 at
 //    D = 256 49 instead of 54; with more two are faster, 64 of 1024 at D = 128 28.3 instead of 31.2,
-//    64 of up to 8192 at D = 256 180 instead of 189);
+//    64 of up to 8192 at D = 256 180 instead of 189).  bf16 has two only where one would have at least
+//    two whole sequences (256 of 100 keys 31.5 instead of 41.5 us, 64 of 300 18 instead of 20; one of
+//    32768 keys, in pieces, 38 instead of 30);
 //  * a sequence (`most` units, the longest) of up to three units is not split: the join
 //    takes as long as two (one of 333 keys: 9.3 instead of 9.5 us), and a longer
 //    one not into more parts than its join, some 2.5 us for 64 rows of
@@ -92,7 +94,8 @@ __device__ __forceinline__ Sequence sequence(const DecodeParams &p, int b) {
 __device__ __forceinline__ uint32_t units_per_workgroup(uint32_t total, uint32_t most, uint32_t grid, uint32_t rows,
                                                         uint32_t few) {
   uint32_t even = (total + grid - 1) / grid;
-  if (grid > 256 && even <= few) even = (total + 255) / 256;
+  const uint32_t alone = (total + 255) / 256;
+  if (grid > 256 && (few ? even <= few : alone < 2 * most)) even = alone;
   const uint32_t least = most <= 3 ? most : min(most, (uint32_t)__builtin_sqrtf((float)(most * rows) * (1.0f / 31.0f)));
   return max(even, max(least, 1u));
 }
@@ -198,11 +201,11 @@ struct VTile {
   }
 };
 
-// Waves per SIMD.  A wave alone on its SIMD reads bf16 as fast as two do, and half
-// the workgroups make half the parts of a split sequence; e4m3 takes twice the
-// arithmetic per byte and is faster with two waves where the registers allow them (64
-// sequences of 4096 keys at D = 128: 92 instead of 104 us).
-constexpr int waves_per_simd(int d, bool fp8, int nt) { return fp8 && d * nt <= 256 ? 2 : 1; }
+// Waves per SIMD that the registers leave room for.  A wave alone reads bf16 as fast as two do, and half
+// the workgroups make half the parts of a split sequence; many short sequences and e4m3, which takes twice the
+// arithmetic per byte, are faster with two (e4m3, 64 sequences of 4096 keys at D = 128: 92
+// instead of 104 us).
+constexpr int waves_per_simd(int d, bool fp8, int nt) { return fp8 ? (d * nt <= 256 ? 2 : 1) : d * nt <= 128 ? 2 : 1; }
 
 // GENERAL: several queries or a cap.  Without it (one token per sequence, no cap) neither is in the code: one sequence
 // of 333 keys 8.2 instead of 8.7 us, 64 of up to 8192 in bf16 175 instead of 176.5.
@@ -249,7 +252,7 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
   }
   most = (uint32_t)__builtin_amdgcn_readfirstlane((int)most);
   const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
-  const uint32_t per = units_per_workgroup(total, most, gridDim.x, (uint32_t)min(ROWS, p.rows), D / 32);
+  const uint32_t per = units_per_workgroup(total, most, gridDim.x, (uint32_t)min(ROWS, p.rows), FP8 ? D / 32 : 0);
   const uint32_t g0 = blockIdx.x * per, g1 = min(g0 + per, total);
   if (g0 >= total) return;  // workgroup-uniform
   int b = __builtin_ctzll(__ballot(incl > g0));
@@ -728,7 +731,9 @@ Plan plan_of(const kfmi_decode_args &a) {
   r.nt = rows <= 16 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
   r.rblocks = (int)((rows + 16 * r.nt - 1) / (16 * r.nt));
   const int64_t units = a.B * a.Hkv * r.rblocks * ((a.max_pages * a.page_size + UNIT - 1) / UNIT);
-  const int64_t round = 256 * waves_per_simd((int)a.D, a.cache_type == KFMI_CACHE_E4M3, r.nt);
+  const bool fp8 = a.cache_type == KFMI_CACHE_E4M3;
+  const bool two = fp8 || a.B * a.Hkv * r.rblocks >= 512;  // bf16: as many heads, or no workgroup has two (units_per_workgroup)
+  const int64_t round = two ? 256 * waves_per_simd((int)a.D, fp8, r.nt) : 256;
   r.grid = units < round ? units : round;
   r.slots = units < 512 ? units : 512;  // for either type of cache
   r.slot_floats = 16 * r.nt * (a.D + 2);
