@@ -718,25 +718,42 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
   }
 }
 
-// Rows of a pass and workgroups of a launch.
+// Blocks of 16 query rows of a pass: all of a head's rows, up to 64 (32 at D = 256).
+int widest(const kfmi_decode_args &a) {
+  const int64_t rows = a.Hq / a.Hkv * a.S;
+  return rows <= 16 ? 1 : rows <= 32 || a.D == 256 ? 2 : 4;
+}
+
+// Workgroups and partial results of a launch.
 struct Plan {
   int nt, rblocks;
-  int64_t grid, slots, slot_floats;
+  int64_t grid;
 };
 
+// Few sequences leave most of the chip idle, and the exchange and the join of 64 rows take 25 us: their
+// rows are dealt to more workgroups in smaller blocks, which read the same keys again, mostly from the caches.  A
+// pass takes half the rows where what is read (of the pages' capacity) is then at most 64 MB, or 256 MB by few
+// heads and blocks (64 rows, one sequence of 2048 keys: 17.6 instead of 44.5 us, one of 16384 40 instead
+// of 76, eight of 2048 35 instead of 49; but eight of 16384 173 instead of 122).
 Plan plan_of(const kfmi_decode_args &a) {
   Plan r{};
-  const int64_t rows = a.Hq / a.Hkv * a.S;
-  const int most = a.D == 128 ? 4 : 2;
-  r.nt = rows <= 16 ? 1 : rows <= 32 || most == 2 ? 2 : 4;
-  r.rblocks = (int)((rows + 16 * r.nt - 1) / (16 * r.nt));
-  const int64_t units = a.B * a.Hkv * r.rblocks * ((a.max_pages * a.page_size + UNIT - 1) / UNIT);
   const bool fp8 = a.cache_type == KFMI_CACHE_E4M3;
-  const bool two = fp8 || a.B * a.Hkv * r.rblocks >= 512;  // bf16: as many heads, or no workgroup has two (units_per_workgroup)
-  const int64_t round = two ? 256 * waves_per_simd((int)a.D, fp8, r.nt) : 256;
+  const int64_t rows = a.Hq / a.Hkv * a.S, capacity = a.max_pages * a.page_size;
+  const int64_t keys = a.window > 0 && a.window < capacity - a.S ? a.window + a.S : capacity;
+  auto blocks = [&](int nt) { return (rows + 16 * nt - 1) / (16 * nt); };
+  r.nt = widest(a);
+  while (r.nt > 1) {
+    const int half = r.nt / 2;
+    const int64_t items = a.B * a.Hkv * blocks(half);
+    const double mb = (double)(items * keys) * (double)(a.D * (fp8 ? 2 : 4)) / (1 << 20);
+    if (!(mb <= 64.0 || (mb <= 256.0 && items <= 64 * half))) break;
+    r.nt = half;
+  }
+  r.rblocks = (int)blocks(r.nt);
+  const int64_t items = a.B * a.Hkv * r.rblocks, units = items * ((capacity + UNIT - 1) / UNIT);
+  // bf16 has two workgroups per CU only where there are as many heads (units_per_workgroup)
+  const int64_t round = fp8 || items >= 512 ? 256 * waves_per_simd((int)a.D, fp8, r.nt) : 256;
   r.grid = units < round ? units : round;
-  r.slots = units < 512 ? units : 512;  // for either type of cache
-  r.slot_floats = 16 * r.nt * (a.D + 2);
   return r;
 }
 
@@ -768,9 +785,12 @@ hipError_t dispatch_decode(const DecodeParams &p, int nt, int64_t grid, hipStrea
 
 }  // namespace
 
+// For any plan of these sizes: two slots of its widest pass for each of at most 512 workgroups.
 int64_t decode_workspace_bytes(const kfmi_decode_args &a) {
-  const Plan r = plan_of(a);
-  return r.slots > 1 ? KFMI_DECODE_COUNTER_BYTES + 2 * r.slots * r.slot_floats * 4 : 0;
+  const int64_t rows = a.Hq / a.Hkv * a.S;
+  const int64_t units = a.B * a.Hkv * ((rows + 15) / 16) * ((a.max_pages * a.page_size + UNIT - 1) / UNIT);
+  const int64_t slots = units < 512 ? units : 512;
+  return slots > 1 ? KFMI_DECODE_COUNTER_BYTES + 2 * slots * 16 * widest(a) * (a.D + 2) * 4 : 0;
 }
 
 hipError_t launch_decode(const kfmi_decode_args &a, hipStream_t stream) {

@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import kernelfuser_amd as kf
+from kernelfuser_amd import _lib
 from helpers import announce
 from serving_ref import attention, held_rows
 
@@ -311,3 +312,22 @@ def test_decode_ratio_of_scale_and_cap_beyond_32_bits(gpu):
     x = _batch([40], (2, 1, 128), 16, "bf16", seed=43)
     x["q"][0, 1] = 0
     _check(x, _decode(_gpu(x, gpu), scale=1e30, softcap=1e-30), softcap=1e-30)
+
+
+@pytest.mark.parametrize("geom,s,nt", [((32, 1, 128), 1, 2), ((8, 2, 128), 8, 2), ((64, 1, 128), 1, 4), ((16, 2, 128), 7, 4),
+                                       ((80, 1, 128), 1, 4), ((32, 1, 256), 1, 2), ((12, 4, 256), 16, 2)])
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_decode_wide_passes(gpu, geom, s, nt, kind):
+    """Page tables of a large capacity, hardly used: the widest passes (32 and 64 rows), also where the rows do not
+    fill them; split and joined, short and empty sequences.  The same rows under a small table, in narrow passes."""
+    announce(f"decode wide {geom} S={s} {kind}")
+    x = _batch([3000, 0, 37, 1], geom, 64, kind, seed=47, s=s)
+    y = _gpu(x, gpu)
+    narrow = _decode(y)
+    _check(x, narrow)
+    wide = dict(y, pages=torch.nn.functional.pad(y["pages"], (0, 2 ** 15), value=-1))
+    with _lib.record_launches() as seen:
+        got = _decode(wide)
+    assert f"decode_kernel<{geom[2]}, {'true' if kind == 'e4m3' else 'false'}, {nt}, " in str(seen.kernels())
+    _check(x, got)
+    _check(x, _decode(wide, window=100, softcap=20.0), 100, 20.0)
