@@ -87,16 +87,16 @@ __device__ __forceinline__ Sequence sequence(const DecodeParams &p, int b) {
 //    32768 keys, in pieces, 38 instead of 30);
 //  * a sequence (`most` units, the longest) of up to three units is not split: the join
 //    takes as long as two (one of 333 keys: 9.3 instead of 9.5 us), and a longer
-//    one not into more parts than its join, some 2.5 us for 64 rows of
-//    parts, leaves worth it: units / parts * 1.2 us + rows * parts / 64 * 2.5 us is least at
-//    parts = sqrt(31 * units / rows) (one of 8192 keys, 32 rows a head: 33 us, 43 in as many parts as
-//    there are units; 64 rows 69 and 84).
+//    one not into more parts than its join, some 0.8 us for 64 rows of
+//    parts, leaves worth it: units / parts * 1.2 us + rows * parts / 64 * 0.8 us is least at
+//    parts = sqrt(96 * units / rows) (one head of 16 rows, 32768 keys at D = 256: 49 us, 94 in as many parts as
+//    there are units, 59 in half of these parts).
 __device__ __forceinline__ uint32_t units_per_workgroup(uint32_t total, uint32_t most, uint32_t grid, uint32_t rows,
                                                         uint32_t few) {
   uint32_t even = (total + grid - 1) / grid;
   const uint32_t alone = (total + 255) / 256;
   if (grid > 256 && (few ? even <= few : alone < 2 * most)) even = alone;
-  const uint32_t least = most <= 3 ? most : min(most, (uint32_t)__builtin_sqrtf((float)(most * rows) * (1.0f / 31.0f)));
+  const uint32_t least = most <= 3 ? most : min(most, (uint32_t)__builtin_sqrtf((float)(most * rows) * (1.0f / 96.0f)));
   return max(even, max(least, 1u));
 }
 
