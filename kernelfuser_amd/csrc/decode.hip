@@ -4,7 +4,7 @@
 // out_i = sum_j softmax_j(cap(q_i . k_j * scale)) v_j over the keys that
 // query i sees.  Every key and value is read once per KV head, so the cache's bytes
 // bound the call: 4 * D bytes (bf16) per key and head against 4 * D * R flops for the R = group * S query rows
-// that share them, at most 64 rows a pass (32 at D = 256).  64 sequences of 4096 keys, 8 heads of D = 128, take
+// that share them, at most 64 rows a pass.  64 sequences of 4096 keys, 8 heads of D = 128, take
 // 169 us (1.07 GB, 6.4 TB/s; a bare read of such pages reaches 6.8), one of 32768 28.4 us, one of 333 8.2; at 32
 // rows in e4m3 the softmax and the conversions bound it instead: 16 sequences of 4096 keys 41 us (137 MB).  The design:
 //
@@ -718,10 +718,12 @@ __global__ __launch_bounds__(NTHR, waves_per_simd(D, FP8, NT)) void decode_kerne
   }
 }
 
-// Blocks of 16 query rows of a pass: all of a head's rows, up to 64 (32 at D = 256).
-int widest(const kfmi_decode_args &a) {
+// Blocks of 16 query rows of a pass: all of a head's rows, up to 64; at D = 256 up to 32 in e4m3 and 16 in bf16,
+// whose 32 need more registers than there are (16 sequences of 4096 keys, 32 rows: 171 us in two passes, 176 in one).
+int widest(const kfmi_decode_args &a, bool fp8) {
   const int64_t rows = a.Hq / a.Hkv * a.S;
-  return rows <= 16 ? 1 : rows <= 32 || a.D == 256 ? 2 : 4;
+  if (rows <= 16 || (a.D == 256 && !fp8)) return 1;
+  return rows <= 32 || a.D == 256 ? 2 : 4;
 }
 
 // Workgroups and partial results of a launch.
@@ -741,7 +743,7 @@ Plan plan_of(const kfmi_decode_args &a) {
   const int64_t rows = a.Hq / a.Hkv * a.S, capacity = a.max_pages * a.page_size;
   const int64_t keys = a.window > 0 && a.window < capacity - a.S ? a.window + a.S : capacity;
   auto blocks = [&](int nt) { return (rows + 16 * nt - 1) / (16 * nt); };
-  r.nt = widest(a);
+  r.nt = widest(a, fp8);
   while (r.nt > 1) {
     const int half = r.nt / 2;
     const int64_t items = a.B * a.Hkv * blocks(half);
@@ -778,8 +780,10 @@ hipError_t launch_decode_s(const DecodeParams &p, int64_t grid, hipStream_t stre
 template <int D, bool FP8>
 hipError_t dispatch_decode(const DecodeParams &p, int nt, int64_t grid, hipStream_t stream) {
   if (nt == 1) return launch_decode_s<D, FP8, 1>(p, grid, stream);
-  if (nt == 2) return launch_decode_s<D, FP8, 2>(p, grid, stream);
-  if constexpr (D == 128) return launch_decode_s<D, FP8, 4>(p, grid, stream);
+  if constexpr (D == 128 || FP8)
+    if (nt == 2) return launch_decode_s<D, FP8, 2>(p, grid, stream);
+  if constexpr (D == 128)
+    if (nt == 4) return launch_decode_s<D, FP8, 4>(p, grid, stream);
   return hipErrorInvalidValue;
 }
 
@@ -790,7 +794,7 @@ int64_t decode_workspace_bytes(const kfmi_decode_args &a) {
   const int64_t rows = a.Hq / a.Hkv * a.S;
   const int64_t units = a.B * a.Hkv * ((rows + 15) / 16) * ((a.max_pages * a.page_size + UNIT - 1) / UNIT);
   const int64_t slots = units < 512 ? units : 512;
-  return slots > 1 ? KFMI_DECODE_COUNTER_BYTES + 2 * slots * 16 * widest(a) * (a.D + 2) * 4 : 0;
+  return slots > 1 ? KFMI_DECODE_COUNTER_BYTES + 2 * slots * 16 * widest(a, true) * (a.D + 2) * 4 : 0;
 }
 
 hipError_t launch_decode(const kfmi_decode_args &a, hipStream_t stream) {
