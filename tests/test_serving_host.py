@@ -276,7 +276,7 @@ def test_logprobs_refusals(logits, ids, top, match):
 
 
 # ---------------------------------------------------------------------------
-# the checkers themselves
+# the 64-bit computations themselves
 # ---------------------------------------------------------------------------
 
 def test_quantise_reference():
